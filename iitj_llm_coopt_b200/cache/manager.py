@@ -30,7 +30,7 @@ different widths, as one flat row per page.
 """
 from __future__ import annotations
 
-from collections import deque
+from collections import Counter, deque
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -53,7 +53,11 @@ class PagePool:
             raise ValueError("a page pool needs at least one page")
         self.num_pages = num_pages
         self.free: deque = deque(range(num_pages))   # FIFO reuse, as engine/block_manager.py:30, 63-66
-        self.held: set = set()
+        self.holders: dict = {}                      # page in use -> how many tables hold it (more than one after a fork)
+
+    @property
+    def held(self) -> set:
+        return set(self.holders)
 
     @property
     def num_free(self) -> int:
@@ -63,14 +67,27 @@ class PagePool:
         if not self.free:
             raise OutOfPages("no free page")
         p = self.free.popleft()
-        self.held.add(p)
+        self.holders[p] = 1
         return p
 
-    def give(self, page: int) -> None:
-        if page not in self.held:
+    def share(self, page: int) -> int:
+        """One more table holds a page that is in use."""
+        if page not in self.holders:
+            raise CacheError(f"page {page} is shared but is not held")
+        self.holders[page] += 1
+        return page
+
+    def give(self, page: int) -> bool:
+        """A table lets go of a page; True if it was the last one and the page is free again."""
+        n = self.holders.get(page)
+        if n is None:
             raise CacheError(f"page {page} is given back but is not held (freed twice?)")
-        self.held.remove(page)
+        if n > 1:
+            self.holders[page] = n - 1
+            return False
+        del self.holders[page]
         self.free.append(page)
+        return True
 
 
 @dataclass
@@ -167,6 +184,11 @@ class CacheManager:
                 # one page more than the pool hands out: the group's padding page.  Rows that only pad a batch to a
                 # size with a captured graph read and write there (the reference keeps such a scratch page too,
                 # engine/engine.py:207-211)
+                if n.bits == 4:
+                    # packed keys and values: a page is one flat row of bytes
+                    g.storage = torch.zeros((len(g.entries), g.pool.num_pages + 1, n.page_bytes(self.page_size, 0)),
+                                            dtype=torch.uint8, device=self.device)
+                    continue
                 if n.value_dim:
                     # values of another width than keys: a page is one flat row, key plane then value plane
                     shape = (len(g.entries), g.pool.num_pages + 1, n.page_elements(self.page_size))
@@ -198,7 +220,7 @@ class CacheManager:
     def bytes_for(needs: list, page_size: int, num_pages: int, itemsize: int, max_requests: int,
                   max_step_tokens: int | None) -> int:
         """Bytes of the paged storage with `num_pages` pages: every cache entry pays for the pages of its group's pool."""
-        return sum(n.page_elements(page_size) * itemsize
+        return sum(n.page_bytes(page_size, itemsize)
                    * (CacheManager.pool_pages(n, page_size, num_pages, max_requests, max_step_tokens) + 1)
                    for n in needs if n.kind == "paged_kv")
 
@@ -256,7 +278,8 @@ class CacheManager:
         return self.stored[request]
 
     def release(self, request) -> int:
-        """Gives back everything the request holds; returns the number of pages returned."""
+        """Gives back everything the request holds; returns the number of pages that are free again (a page that a
+        fork still holds is not)."""
         if request not in self.stored:
             raise CacheError(f"request {request!r} is not admitted (released twice?)")
         n = 0
@@ -266,8 +289,7 @@ class CacheManager:
             table = g.tables.pop(request)
             for p in table:
                 if p >= 0:
-                    g.pool.give(p)
-                    n += 1
+                    n += g.pool.give(p)
             g.matrix[slot, :len(table)] = 0
             g.lengths[slot] = 0
         self.free_slots.append(self.slot_of.pop(request))
@@ -394,6 +416,8 @@ class CacheManager:
             keep = g.pages_for(total_tokens)
             if any(p < 0 for p in table[g.first_needed_page(total_tokens):keep]):
                 raise CacheError("truncate would need pages that a window already gave back")
+            if total_tokens % self.page_size and keep <= len(table) and g.pool.holders.get(table[keep - 1], 0) > 1:
+                raise CacheError("truncate would go on writing in a page that a fork shares")
             old = len(table)
             while len(table) > keep:
                 p = table.pop()
@@ -404,6 +428,48 @@ class CacheManager:
                 g.lengths[self.slot_of[request]] = keep
         self.stored[request] = min(self.stored[request], total_tokens)
         self._set_room(request)
+
+    # ---- forks -----------------------------------------------------------------------------
+    # A fork starts as a request whose first tokens are another's: it holds the same full pages (nobody writes in a full
+    # page again), and of the page that both would go on writing a copy of its own.
+    def can_fork(self, parent, tokens: int) -> bool:
+        """True if `fork` can give a new request the parent's first `tokens` tokens: they are stored and their pages still
+        there, a request slot and, where the tokens end inside a page, a page per group are free, and no layer keeps state (a
+        state holds all tokens so far: it cannot be taken back to fewer)."""
+        if not self.free_slots or not 0 < tokens <= self.stored.get(parent, 0):
+            return False
+        for g in self.groups:
+            if not isinstance(g, PagedGroup):
+                return False
+            table = g.tables[parent]
+            if any(p < 0 for p in table[g.first_needed_page(tokens):g.pages_for(tokens)]):
+                return False
+            if tokens % self.page_size and not g.pool.num_free:
+                return False
+        return True
+
+    def fork(self, parent, child, tokens: int) -> list:
+        """Admits `child` with the parent's first `tokens` tokens.  Returns the pages whose contents the caller has to copy before
+        the child's first step, as (group, source page, destination page); `ModelRunner.fork` does both."""
+        if child in self.stored:
+            raise CacheError(f"request {child!r} is already admitted")
+        if not self.can_fork(parent, tokens):
+            raise CacheError(f"request {parent!r} cannot be forked after {tokens} tokens")
+        slot = self.admit(child)
+        full, copies = tokens // self.page_size, []
+        for gi in self.paged:
+            g = self.groups[gi]
+            source, table = g.tables[parent], g.tables[child]
+            table.extend(p if p < 0 else g.pool.share(p) for p in source[:full])
+            if tokens % self.page_size:
+                table.append(g.pool.take())
+                copies.append((gi, source[full], table[full]))
+            g.columns(len(table))
+            g.matrix[slot, :len(table)] = [max(p, 0) for p in table]
+            g.lengths[slot] = len(table)
+        self.stored[child] = tokens
+        self._set_room(child)
+        return copies
 
     # ---- what the step function needs ----------------------------------------------------
     def table(self, group: int, request) -> list:
@@ -425,19 +491,17 @@ class CacheManager:
 
     # ---- invariants (tests) --------------------------------------------------------------
     def check(self) -> None:
-        """Every page is either free or in exactly one table; slots likewise."""
+        """Every page is either free or in as many tables as it has holders (one, without forks); slots in exactly one."""
         for gi in self.paged:
             g = self.groups[gi]
             in_tables = [p for t in g.tables.values() for p in t if p >= 0]
-            if len(in_tables) != len(set(in_tables)):
-                raise CacheError(f"group {gi}: a page is held twice")
-            if set(in_tables) != g.pool.held:
+            if Counter(in_tables) != g.pool.holders:
                 raise CacheError(f"group {gi}: tables and pool disagree about held pages")
             free = list(g.pool.free)
             if len(free) != len(set(free)) or set(free) & g.pool.held:
                 raise CacheError(f"group {gi}: free list is inconsistent")
-            if len(free) + len(in_tables) != g.pool.num_pages:
-                raise CacheError(f"group {gi}: {g.pool.num_pages - len(free) - len(in_tables)} pages are lost")
+            if len(free) + len(g.pool.holders) != g.pool.num_pages:
+                raise CacheError(f"group {gi}: {g.pool.num_pages - len(free) - len(g.pool.holders)} pages are lost")
             if set(g.tables) != set(self.stored):
                 raise CacheError(f"group {gi}: tables exist for other requests than the admitted ones")
             rows = np.zeros_like(g.matrix)

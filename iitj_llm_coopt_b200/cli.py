@@ -259,6 +259,7 @@ def main(argv=None) -> int:
     ap.add_argument("--max-model-len", type=int, default=32768)
     ap.add_argument("--gpu-memory-utilization", type=float, default=0.9)
     ap.add_argument("--dtype", default="bfloat16", help="bfloat16 or float32")
+    ap.add_argument("--kv-cache", default="model", choices=["model", "int4"], help="keys and values in --dtype, or packed to 4-bit codes")
     args = ap.parse_args(argv)
 
     # a baseline workload brings its shape, seed and token budget; what the command line gives wins
@@ -284,7 +285,8 @@ def main(argv=None) -> int:
     from . import EngineConfig, build_engine
     ec = EngineConfig(dtype=args.dtype, page_size=args.page_size, num_pages=args.num_pages, kv_gb=args.kv_gb,
                       gpu_memory_utilization=args.gpu_memory_utilization, max_model_len=args.max_model_len,
-                      max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_num_batched_tokens, seed=args.seed)
+                      max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_num_batched_tokens, seed=args.seed,
+                      kv_cache=args.kv_cache)
     if args.model is not None:
         engine = build_engine(args.model, ec)
     else:

@@ -14,6 +14,8 @@ DTYPE_ALIASES = {
     "float32": "float32", "fp32": "float32", "float": "float32",
 }
 
+KV_CACHES = ("model", "int4")
+
 
 def canonical_dtype(name) -> str:
     key = str(name).replace("torch.", "").lower()
@@ -37,10 +39,13 @@ class EngineConfig:
     cuda_graphs: bool = True            # replay decode-only steps from captured graphs
     lookahead: bool = True              # launch the next decode step before the host has read this one's tokens
     device: str = "cuda:0"
+    kv_cache: str = "model"             # "model": keys and values in `dtype`; "int4": packed to 4-bit codes (csrc/kv4.cuh)
 
     def __post_init__(self):
         self.dtype = canonical_dtype(self.dtype)
         if self.page_size <= 0:
             raise ValueError("page_size must be positive")
+        if self.kv_cache not in KV_CACHES:
+            raise ValueError(f"kv_cache {self.kv_cache!r} is not known: use one of {', '.join(KV_CACHES)}")
         if self.max_num_seqs <= 0 or self.max_num_batched_tokens <= 0:
             raise ValueError("max_num_seqs and max_num_batched_tokens must be positive")

@@ -47,6 +47,8 @@ class CacheNeed:
         key plane [kv_heads, page, head_dim] followed by the value plane [kv_heads, page, value_dim].
         shared_value: the values are the leading `value_dim` numbers of the key rows themselves (one latent row per
         token that serves as key and as value); a page is then the key plane alone.
+        bits: 0 keeps numbers of the engine's type; 4 packs keys and values into 4-bit codes (csrc/kv4.cuh): a page is
+        one flat row of bytes, `head_dim` a multiple of 32, the page size a multiple of 4.
     kind "state":    a fixed-size record per request (`state_shape`, `state_dtype`).
     kind "none":     nothing.
     Layers whose needs compare equal share one group of the cache manager.
@@ -59,12 +61,19 @@ class CacheNeed:
     state_dtype: str = "float32"
     value_dim: int = 0
     shared_value: bool = False
+    bits: int = 0
 
     def page_elements(self, page_size: int) -> int:
         """Numbers one page of one cache entry holds."""
         if self.shared_value:
             return self.kv_heads * page_size * self.head_dim
         return self.kv_heads * page_size * (self.head_dim + (self.value_dim or self.head_dim))
+
+    def page_bytes(self, page_size: int, itemsize: int) -> int:
+        """Bytes one page of one cache entry takes; `itemsize`: of the engine's type."""
+        if self.bits == 4:
+            return self.kv_heads * page_size * (self.head_dim // 32) * 40
+        return self.page_elements(page_size) * itemsize
 
 
 @dataclass(frozen=True)

@@ -1,0 +1,170 @@
+// Attention over the packed key/value cache (format: kv4.cuh): the general kernel.
+//
+// Any head size (a multiple of 32 up to 256), any page size (a multiple of 4), both engine types, any mix of prompt portions and
+// single tokens: one block a token row and key/value head, for up to eight of the group's query heads at a time.  Every number of the
+// cache is taken apart once per block, as z + s n in float32, and enters float32 products.
+//
+//   scores   a lane is a key: it reads its key's words and adds q . k for the block's query heads, q broadcast from shared memory
+//   softmax  running maximum and sum a head and warp (warp w takes the 32-key chunks w, w + 4, ..., so the four warps see different keys)
+//   values   a lane is four numbers of the value head (a half-word of codes), the chunk's probabilities broadcast from shared memory
+// and at the end the four warps' sums are joined.  Keys outside [lo, pos] are not read.
+#include "kv4.cuh"
+
+namespace {
+
+constexpr int kGenThreads = 128, kGenWarps = 4, kGenHeads = 8;
+
+template <typename T> __device__ __forceinline__ T of_float(float v) { return from_f32<T>(v); }
+
+template <typename T>
+__global__ void __launch_bounds__(kGenThreads)
+attn_kv4_general_kernel(const T* __restrict__ q, int q_stride, const uint8_t* __restrict__ cache, const int* __restrict__ block_table,
+                        int table_width, const int* __restrict__ token_request, const int* __restrict__ positions, T* __restrict__ out,
+                        int out_stride, int heads, int kv_heads, int head_dim, int page_size, int window, float sl) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ __align__(16) float sq[kGenHeads][kKv4MaxDim];
+    __shared__ float sp[kGenWarps][kGenHeads][32];
+    __shared__ float sm[kGenWarps][kGenHeads], sl_sum[kGenWarps][kGenHeads];
+    const int t = blockIdx.x, hk = blockIdx.y, D = head_dim, G = D / 32, group = heads / kv_heads;
+    const int h0 = hk * group + blockIdx.z * kGenHeads, nh = min(kGenHeads, group - (int)blockIdx.z * kGenHeads);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int pos = positions[t], lo = window > 0 ? max(0, pos - window + 1) : 0;
+    const int* table = block_table + (size_t)token_request[t] * table_width;
+    const size_t block_bytes = kv4_block_bytes(page_size, G);
+    for (int i = threadIdx.x; i < kGenHeads * D; i += kGenThreads) {
+        const int h = i / D, c = i - h * D;
+        sq[h][c] = h < nh ? to_f32(q[(size_t)t * q_stride + (size_t)(h0 + h) * D + c]) * sl : 0.f;       // (scores in log2 units)
+    }
+    __syncthreads();
+    // this lane's value numbers: half-words lane and lane + 32 of a row
+    const int units = 8 * G;
+    float o[2][kGenHeads][4], m[kGenHeads], l[kGenHeads];
+#pragma unroll
+    for (int h = 0; h < kGenHeads; ++h) {
+        m[h] = -INFINITY; l[h] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][h][e] = o[1][h][e] = 0.f;
+    }
+    for (int k0 = lo + warp * 32; k0 <= pos; k0 += kGenWarps * 32) {
+        const int n = min(32, pos + 1 - k0), key = k0 + min(lane, n - 1);
+        const int lp = key / page_size, off = key - lp * page_size;
+        const uint8_t* block = cache + ((size_t)table[lp] * kv_heads + hk) * block_bytes;
+        const uint32_t* codes = reinterpret_cast<const uint32_t*>(block + (size_t)off * 16 * G);
+        const uint32_t* par = reinterpret_cast<const uint32_t*>(block + kv4_key_par(page_size, G) + (size_t)off * 4 * G);
+        float s[kGenHeads];
+#pragma unroll
+        for (int h = 0; h < kGenHeads; ++h) s[h] = 0.f;
+        for (int g = 0; g < G; ++g) {
+            const uint32_t p = par[g];
+            const float step = kv4_step(p), zero = kv4_zero(p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = codes[j * G + g];
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = fmaf(step, (float)((w >> kv4_bit(e)) & 15u), zero);
+#pragma unroll
+                for (int h = 0; h < kGenHeads; ++h) {
+                    const float4 a = *reinterpret_cast<const float4*>(&sq[h][32 * g + 8 * j]), b = *reinterpret_cast<const float4*>(&sq[h][32 * g + 8 * j + 4]);
+                    s[h] += ((a.x * x[0] + a.y * x[1]) + (a.z * x[2] + a.w * x[3])) + ((b.x * x[4] + b.y * x[5]) + (b.z * x[6] + b.w * x[7]));
+                }
+            }
+        }
+        __syncwarp();                                    // the chunk before is done with sp
+#pragma unroll
+        for (int h = 0; h < kGenHeads; ++h) {
+            const float v = lane < n ? s[h] : -INFINITY;
+            const float top = fmaxf(m[h], warp_max(v));
+            const float mu = top == -INFINITY ? 0.f : top;              // (every score -inf so far: nothing to be relative to)
+            const float f = exp2f(m[h] - mu), p = lane < n ? exp2f(v - mu) : 0.f;
+            m[h] = top;
+            l[h] = l[h] * f + p;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { o[0][h][e] *= f; o[1][h][e] *= f; }
+            sp[warp][h][lane] = p;
+        }
+        __syncwarp();
+        for (int i = 0; i < n; ++i) {
+            const int kk = k0 + i, vp = kk / page_size, voff = kk - vp * page_size;
+            const uint8_t* vb = cache + ((size_t)table[vp] * kv_heads + hk) * block_bytes;
+            const uint16_t* vc = reinterpret_cast<const uint16_t*>(vb + kv4_value_codes(page_size, G) + (size_t)voff * 16 * G);
+            const uint32_t* vpar = reinterpret_cast<const uint32_t*>(vb + kv4_value_par(page_size, G) + (size_t)voff * 4 * G);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int u = lane + 32 * r;
+                if (u < units) {
+                    const uint32_t w = vc[u], p4 = vpar[u % G];
+                    const float step = kv4_step(p4), zero = kv4_zero(p4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = fmaf(step, (float)((w >> (4 * e)) & 15u), zero);
+#pragma unroll
+                        for (int h = 0; h < kGenHeads; ++h) o[r][h][e] = fmaf(sp[warp][h][i], x, o[r][h][e]);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < kGenHeads; ++h) {
+        l[h] = warp_sum(l[h]);
+        if (lane == 0) { sm[warp][h] = m[h]; sl_sum[warp][h] = l[h]; }
+    }
+    __syncthreads();
+    // joined over the warps, one after another, into the query rows' place
+    for (int w = 0; w < kGenWarps; ++w) {
+        if (warp == w) {
+            for (int h = 0; h < nh; ++h) {
+                const float top = fmaxf(fmaxf(sm[0][h], sm[1][h]), fmaxf(sm[2][h], sm[3][h]));
+                const float f = sm[w][h] == -INFINITY ? (sl_sum[w][h] == 0.f ? 0.f : 1.f) : exp2f(sm[w][h] - top);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int u = lane + 32 * r;
+                    if (u < units) {
+                        const int c = u / G, g = u - c * G, at = 32 * g + 8 * (c >> 1) + (c & 1);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float v = 0.f;
+                            // (a loop over h with o[r][h] in registers: selected by comparison)
+#pragma unroll
+                            for (int hh = 0; hh < kGenHeads; ++hh) if (hh == h) v = o[r][hh][e];
+                            sq[h][at + 2 * e] = (w == 0 ? 0.f : sq[h][at + 2 * e]) + f * v;
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < nh * D; i += kGenThreads) {
+        const int h = i / D, c = i - h * D;
+        const float top = fmaxf(fmaxf(sm[0][h], sm[1][h]), fmaxf(sm[2][h], sm[3][h]));
+        float sum = 0.f;
+        for (int w = 0; w < kGenWarps; ++w) sum += sl_sum[w][h] * (sm[w][h] == -INFINITY ? (sl_sum[w][h] == 0.f ? 0.f : 1.f) : exp2f(sm[w][h] - top));
+        out[(size_t)t * out_stride + (size_t)(h0 + h) * D + c] = of_float<T>(sq[h][c] / sum);
+    }
+}
+
+}  // namespace
+
+// q: [tokens, q_stride], head h at columns [h * head_dim, ...); cache: pages of kv_heads blocks (kv4.cuh).
+LLM_API int llm_attention_kv4_general(const void* q, int q_stride, const void* cache, const int* block_table, int table_width,
+                                      const int* token_request, const int* positions, void* out, int out_stride, int dtype, int tokens, int heads,
+                                      int kv_heads, int head_dim, int page_size, int window, float scale, cudaStream_t stream) {
+    if (tokens == 0) return 0;
+    if (!kv4_geometry(head_dim, page_size) || kv_heads <= 0 || heads % kv_heads)
+        LLM_FAIL(-1, "attention_kv4: heads %d / kv_heads %d / head_dim %d / page %d not supported", heads, kv_heads, head_dim, page_size);
+    const int tiles = (heads / kv_heads + kGenHeads - 1) / kGenHeads;
+    if (kv_heads > 65535 || tiles > 65535) LLM_FAIL(-1, "attention_kv4: too many heads");
+    return llm_dispatch_dtype(dtype, [&](auto tag) {
+        using T = decltype(tag);
+        llm_launch(attn_kv4_general_kernel<T>, dim3(tokens, kv_heads, tiles), kGenThreads, 0, stream, (const T*)q, q_stride, (const uint8_t*)cache,
+                   block_table, table_width, token_request, positions, (T*)out, out_stride, heads, kv_heads, head_dim, page_size, window,
+                   scale * 1.4426950408889634f);
+        LLM_CHECK_LAUNCH("attention_kv4");
+        return 0;
+    });
+}
+
+LLM_TRACE_EXPORT(attention_kv4)

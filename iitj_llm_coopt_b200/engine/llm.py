@@ -15,7 +15,7 @@ import torch
 
 from ..cache import CacheManager
 from ..config import EngineConfig, load_config
-from ..models.decoder import build_model, cache_needs
+from ..models.decoder import build_model, cache_needs, packed_cache_needs
 from ..sampling import Sampler, SamplingParams
 from ..weights import load_parameters, random_parameters
 from .engine import Engine
@@ -80,7 +80,7 @@ def build_engine(model: str | None = None, engine_config: EngineConfig | None = 
             params = random_parameters(arch, spec, random_seed or 0, dtype, device=device)
         net.load_parameters(params)
         del params
-        needs = cache_needs(spec)
+        needs = packed_cache_needs(spec, ec.page_size) if ec.kv_cache == "int4" else cache_needs(spec)
         itemsize = 2 if dtype == torch.bfloat16 else 4
         step_tokens = ec.max_num_batched_tokens
 
@@ -125,18 +125,19 @@ class LLM:
                  page_size: int = 16, num_pages: int | None = None, kv_gb: float | None = None,
                  gpu_memory_utilization: float = 0.9, max_model_len: int = 32768, max_num_seqs: int = 256,
                  max_num_batched_tokens: int = 2048, seed: int = 0, device: str = "cuda:0", kernels=None,
-                 cuda_graphs: bool = True, lookahead: bool = True):
+                 cuda_graphs: bool = True, lookahead: bool = True, kv_cache: str = "model"):
         ec = EngineConfig(dtype=dtype, page_size=page_size, num_pages=num_pages, kv_gb=kv_gb,
                           gpu_memory_utilization=gpu_memory_utilization, max_model_len=max_model_len,
                           max_num_seqs=max_num_seqs, max_num_batched_tokens=max_num_batched_tokens, seed=seed,
-                          device=device, cuda_graphs=cuda_graphs, lookahead=lookahead)
+                          device=device, cuda_graphs=cuda_graphs, lookahead=lookahead, kv_cache=kv_cache)
         self.engine = build_engine(model, ec, config=config, random_seed=random_seed, kernels=kernels)
 
     def generate(self, prompt_token_ids, sampling_params=None, on_output=None) -> list:
         """prompt_token_ids: a list of prompts (each a list of token ids).  sampling_params:
         one SamplingParams for all, or one per prompt.  `on_output(sequence, new_token_ids, finished)` is
         called as tokens arrive, as the reference's Sequence.on_output (engine/engine.py:40, 483-484).
-        Returns RequestOutputs in order."""
+        Returns RequestOutputs in order; a prompt whose SamplingParams ask for n completions has n of them, one after
+        the other, which share the prompt's cache pages."""
         if prompt_token_ids and isinstance(prompt_token_ids[0], int):
             prompt_token_ids = [prompt_token_ids]
         n = len(prompt_token_ids)
@@ -147,8 +148,8 @@ class LLM:
         if len(sampling_params) != n:
             raise ValueError("one SamplingParams per prompt, or one for all")
         t0 = time.perf_counter()
-        seqs = [self.engine.new_sequence(p, sp.max_tokens, sp.temperature, sp.ignore_eos, sp.seed, on_output)
-                for p, sp in zip(prompt_token_ids, sampling_params)]
+        seqs = [s for p, sp in zip(prompt_token_ids, sampling_params)
+                for s in self.engine.new_sequences(sp.n, p, sp.max_tokens, sp.temperature, sp.ignore_eos, sp.seed, on_output)]
         self.engine.run_until_done()
         return [RequestOutput(request_id=s.seq_id, prompt_token_ids=s.tokens[:s.prompt_len],
                               token_ids=s.tokens[s.prompt_len:], finish_reason=s.finish_reason,

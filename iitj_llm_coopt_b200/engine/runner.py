@@ -157,6 +157,35 @@ class ModelRunner:
         step = 8 if b <= 64 else 16 if b <= 128 else 32
         return -(-b // step) * step
 
+    # ---- the cache's contents ----------------------------------------------------------
+    def fork(self, parent, child, tokens: int) -> None:
+        """Admits `child` to the cache with the parent's first `tokens` tokens (CacheManager.fork) and copies the pages that
+        the two do not share, in every layer's entry, on the current stream."""
+        pairs: dict = {}
+        for group, src, dst in self.cache.fork(parent, child, tokens):
+            pairs.setdefault(group, []).append((src, dst))
+        for group, p in pairs.items():
+            self.model.k.copy_pages(self.cache.groups[group].storage, p)
+
+    def read_cache(self, request, entry: int, start: int = 0, end: int | None = None) -> torch.Tensor:
+        """Keys and values that a cache entry holds of a request's tokens [start, end) (default: all stored), as float32
+        [tokens, 2, kv_heads, head_dim]; a packed entry's numbers are what its codes stand for."""
+        cache = self.cache
+        stored = cache.num_tokens(request)
+        end = stored if end is None else end
+        if not 0 <= start <= end <= stored:
+            raise ValueError(f"tokens [{start}, {end}) are not among the {stored} that request {request!r} has stored")
+        group, view = cache.view(entry)
+        if group is None or group not in cache.paged or cache.groups[group].need.value_dim:
+            raise CacheError(f"cache entry {entry} does not keep keys and values of one size in pages")
+        need = cache.groups[group].need
+        slots = torch.tensor(cache.slots(group, request, start, end), dtype=torch.int32).to(self.device)
+        if need.bits == 4:
+            out = torch.empty((end - start, 2, need.kv_heads, need.head_dim), dtype=torch.float32, device=self.device)
+            return self.model.k.kv4_read(view, slots, out, need.kv_heads, need.head_dim)
+        slots = slots.long()
+        return view[slots // cache.page_size, :, :, slots % cache.page_size].float()
+
     # ---- the step --------------------------------------------------------------------
     def step(self, entries: list, prev_ids=None):
         """`prev_ids`: the previous step's sampled ids on the device, for entries with `source_rows`."""

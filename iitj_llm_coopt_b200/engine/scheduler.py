@@ -49,6 +49,7 @@ class Sequence:
     finished: bool = False
     finish_reason: str | None = None
     num_preemptions: int = 0
+    branches: list = field(default_factory=list)    # sequences of the same prompt that fork from this one once it is computed
     pending_row: int | None = None      # row of the step in flight whose sampled id is this sequence's last token
 
     def __post_init__(self):

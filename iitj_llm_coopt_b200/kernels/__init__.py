@@ -45,6 +45,12 @@ _SIGNATURES = {
     "llm_rope_table": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_float, _c_void_p],
     "llm_rope_store": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_int, ctypes.c_longlong, _c_void_p],
+    "llm_rope_store_kv4": [_c_void_p, _c_void_p, _c_int, ctypes.c_longlong, _c_void_p, ctypes.c_longlong, _c_void_p, _c_void_p, _c_void_p,
+                           _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p],
+    "llm_kv4_read": [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p],
+    "llm_attention_kv4_general": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
+                                  _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p],
+    "llm_copy_pages": [_c_void_p, _c_int, ctypes.c_longlong, ctypes.c_longlong, ctypes.POINTER(_c_int), _c_int, _c_void_p],
     "llm_silu_mul": [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p],
     "llm_scale_f32": [_c_void_p, _c_float, ctypes.c_longlong, _c_void_p],
     "llm_sum_parts": [_c_void_p, _c_void_p, _c_int, _c_int, ctypes.c_longlong, _c_void_p],
@@ -691,6 +697,94 @@ class Kernels:
                    parts.splits if parts is not None else 0, parts.stride if parts is not None else 0, self._stream())
         return qkv
 
+    # ---- packed keys and values, pages of a cache ------------------------------------
+    @staticmethod
+    def _kv4_page_size(name, cache_layer, kv_heads, head_dim) -> int:
+        """Tokens a page of a packed cache layer [pages, bytes] holds (csrc/kv4.cuh)."""
+        _check(cache_layer, name + ".cache", torch.uint8, 2)
+        _need(head_dim % 32 == 0 and 32 <= head_dim <= 256, f"{name}: head_dim {head_dim} is not a multiple of 32 up to 256")
+        token = kv_heads * (head_dim // 32) * 40
+        _need(kv_heads > 0 and cache_layer.shape[1] % (4 * token) == 0 and cache_layer.shape[1] > 0,
+              f"{name}.cache: pages of {cache_layer.shape[1]} bytes are no multiple of 4 tokens of {kv_heads} heads of {head_dim} numbers")
+        _need(cache_layer.data_ptr() % 16 == 0, f"{name}.cache: not on a 16-byte boundary")
+        return cache_layer.shape[1] // token
+
+    def rope_store_kv4(self, qkv, tables, slots, cache_layer, heads, kv_heads, head_dim, rotary_dim, q_out=None):
+        """`rope_store` into a packed cache: rotates the queries, rotates and packs the keys, packs the values and stores both in
+        every token's cache slot (a slot below 0: nowhere).
+
+        cache_layer: uint8 [pages, bytes] (csrc/kv4.cuh); slots may be None (rotate only).  tables: (cos, sin) of `rope_tables`
+        (None with rotary_dim 0).  `qkv` may be a PartialSums of up to eight parts: they are added on the way.  `q_out`
+        [tokens, heads * head_dim] receives the queries; without it they are rotated in place in qkv, whose keys and values stay as
+        they are.  Returns the tensor that holds the rotated queries."""
+        parts = None
+        if isinstance(qkv, PartialSums):
+            if qkv.splits <= 8 and qkv.stride % 4 == 0:
+                parts, qkv = qkv, qkv.out
+            else:
+                qkv = qkv.sum()
+        _check(qkv, "rope_store_kv4.qkv", tuple(DTYPE_CODE), 2)
+        tokens = qkv.shape[0]
+        _need(heads > 0 and kv_heads > 0 and qkv.shape[1] == (heads + 2 * kv_heads) * head_dim,
+              "rope_store_kv4.qkv: width is not (heads+2*kv_heads)*head_dim")
+        _need(0 <= rotary_dim <= head_dim and rotary_dim % 8 == 0, f"rope_store_kv4: rotary_dim {rotary_dim} is not a multiple of 8 up to {head_dim}")
+        _need(head_dim % 32 == 0 and 32 <= head_dim <= 256, f"rope_store_kv4: head_dim {head_dim} is not a multiple of 32 up to 256")
+        cos = sin = None
+        if rotary_dim:
+            _need(tables is not None, "rope_store_kv4: a rotation needs its tables")
+            cos, sin = tables
+            _check(cos, "rope_store_kv4.cos", torch.float32, 2)
+            _check(sin, "rope_store_kv4.sin", torch.float32, 2)
+            _need(cos.shape == (tokens, rotary_dim // 2) and sin.shape == cos.shape, "rope_store_kv4: wrong table shape")
+        page_size = 4
+        if slots is not None:
+            _check(slots, "rope_store_kv4.slots", torch.int32, 1)
+            _need(slots.shape[0] == tokens, "rope_store_kv4.slots: one per token")
+            page_size = self._kv4_page_size("rope_store_kv4", cache_layer, kv_heads, head_dim)
+        if q_out is not None:
+            _check(q_out, "rope_store_kv4.q_out", qkv.dtype, 2)
+            _need(q_out.shape == (tokens, heads * head_dim), "rope_store_kv4.q_out: wrong shape")
+        else:
+            q_out = qkv
+        for name, t in (("qkv", qkv), ("q_out", q_out), ("cos", cos), ("sin", sin)):
+            _need(t is None or t.data_ptr() % 16 == 0, f"rope_store_kv4.{name}: not on a 16-byte boundary")
+        self._call("llm_rope_store_kv4", None if parts is not None else _ptr(qkv), _ptr(parts.parts) if parts is not None else None,
+                   parts.splits if parts is not None else 0, parts.stride if parts is not None else 0, _ptr(q_out), q_out.shape[1],
+                   _ptr(cos), _ptr(sin), _ptr(slots), _ptr(cache_layer) if slots is not None else None, DTYPE_CODE[qkv.dtype], tokens,
+                   heads, kv_heads, head_dim, rotary_dim, page_size, self._stream())
+        return q_out
+
+    def kv4_read(self, cache_layer, slots, out, kv_heads, head_dim):
+        """out[i] = the key and the value of cache slot slots[i] of a packed cache layer, as numbers: [n, 2, kv_heads, head_dim] in
+        one of the engine's types (a slot below 0 reads as zeros)."""
+        page_size = self._kv4_page_size("kv4_read", cache_layer, kv_heads, head_dim)
+        _check(slots, "kv4_read.slots", torch.int32, 1)
+        _check(out, "kv4_read.out", tuple(DTYPE_CODE), 4)
+        _need(tuple(out.shape) == (slots.shape[0], 2, kv_heads, head_dim), "kv4_read.out: wrong shape")
+        _need(out.data_ptr() % 16 == 0, "kv4_read.out: not on a 16-byte boundary")
+        self._call("llm_kv4_read", _ptr(cache_layer), _ptr(slots), _ptr(out), DTYPE_CODE[out.dtype], slots.shape[0], kv_heads, head_dim,
+                   page_size, self._stream())
+        return out
+
+    def copy_pages(self, storage, pairs):
+        """storage[:, dst] = storage[:, src] for every (src, dst) of `pairs` (page ids, a list on the host), all at once: no
+        destination may be another pair's destination or anybody's source.  storage: [entries, pages, ...] of any type."""
+        _check(storage, "copy_pages.storage")
+        _need(storage.dim() >= 2, f"copy_pages.storage: want [entries, pages, ...], got shape {tuple(storage.shape)}")
+        pairs = [(int(a), int(b)) for a, b in pairs]
+        pages = storage.shape[1]
+        for a, b in pairs:
+            _need(0 <= a < pages and 0 <= b < pages, f"copy_pages: ({a}, {b}) are not both among the pool's {pages} pages")
+        targets = {b for _, b in pairs}
+        _need(len(targets) == len(pairs), "copy_pages: a page is the destination of two copies")
+        _need(not targets & {a for a, _ in pairs}, "copy_pages: a page is the source of one copy and the destination of another")
+        if pairs and storage.numel():
+            flat = (_c_int * (2 * len(pairs)))(*(x for pair in pairs for x in pair))
+            self._call("llm_copy_pages", _ptr(storage), storage.shape[0], pages, storage[0, 0].numel() * storage.element_size(), flat,
+                       len(pairs), self._stream())
+            self.launches += (len(pairs) - 1) // 256          # a launch carries 256 pairs
+        return storage
+
     def silu_mul(self, gu, act):
         _check(gu, "silu_mul.gu", tuple(DTYPE_CODE), 2)
         _check(act, "silu_mul.act", gu.dtype, 2)
@@ -781,6 +875,29 @@ class Kernels:
                    meta.block_table.shape[1], _ptr(meta.token_request), _ptr(meta.positions), _ptr(out),
                    out.shape[1], DTYPE_CODE[qkv.dtype], tokens, heads, kv_heads, head_dim, page_size,
                    int(window), float(scale), self._stream())
+        return out
+
+    def attention_kv4(self, q, cache_layer, meta, out, heads, kv_heads, head_dim, window: int = 0, scale: float = 0.0):
+        """`attention` over a packed cache layer (uint8 [pages, bytes], csrc/kv4.cuh): causal attention of every token of `q` (query
+        heads first in each row) over the numbers that its request's codes stand for."""
+        _check(q, "attention_kv4.q", tuple(DTYPE_CODE), 2)
+        _check(out, "attention_kv4.out", q.dtype, 2)
+        tokens = q.shape[0]
+        page_size = self._kv4_page_size("attention_kv4", cache_layer, kv_heads, head_dim)
+        _need(heads > 0 and heads % kv_heads == 0, f"attention_kv4: heads {heads} is not a multiple of kv_heads {kv_heads}")
+        _need(q.shape[1] >= heads * head_dim, "attention_kv4.q: row too narrow")
+        _need(out.shape == (tokens, heads * head_dim), "attention_kv4.out: wrong shape")
+        _check(meta.block_table, "attention_kv4.block_table", torch.int32, 2)
+        _check(meta.token_request, "attention_kv4.token_request", torch.int32, 1)
+        _check(meta.positions, "attention_kv4.positions", torch.int32, 1)
+        _need(meta.token_request.shape[0] == tokens and meta.positions.shape[0] == tokens,
+              "attention_kv4: one token_request and one position per token")
+        if not scale:
+            scale = 1.0 / math.sqrt(head_dim)
+        if tokens:
+            self._call("llm_attention_kv4_general", _ptr(q), q.shape[1], _ptr(cache_layer), _ptr(meta.block_table), meta.block_table.shape[1],
+                       _ptr(meta.token_request), _ptr(meta.positions), _ptr(out), out.shape[1], DTYPE_CODE[q.dtype], tokens, heads, kv_heads,
+                       head_dim, page_size, int(window), float(scale), self._stream())
         return out
 
     def _attention_f32_takes(self, qkv, cache_layer, meta, out, heads, kv_heads, head_dim) -> bool:

@@ -9,9 +9,12 @@ Forward formulas in the reference's order: engine/model.py:181-213.
 """
 from __future__ import annotations
 
+import dataclasses
+
 import torch
 
 from .. import parts as P
+from ..config.errors import ConfigError
 from ..parts.base import delta_for
 from ..parts.stream_join import ORIGIN
 
@@ -84,6 +87,26 @@ def cache_needs(spec) -> list:
             raise ValueError(f"run order reads cache entry {call.cache} that no call writes")
     n = max(entries) + 1 if entries else 0
     return [entries.get(i, CacheNeed()) for i in range(n)]
+
+
+def packed_cache_needs(spec, page_size: int) -> list:
+    """`cache_needs` with every key/value entry packed to 4-bit codes (`EngineConfig.kv_cache` "int4").  ConfigError for a model
+    with a layer whose mixer has no packed form, or sizes that the packed pages do not take."""
+    needs = cache_needs(spec)
+    if not any(n.kind == "paged_kv" for n in needs):
+        raise ConfigError("kv_cache 'int4': this model keeps no keys and values in pages")
+    if page_size % 4:
+        raise ConfigError(f"kv_cache 'int4': page_size {page_size} is not a multiple of 4")
+    for call in spec.order:
+        for _name, family, part_spec, cls in layer_parts(spec.layers[call.layer]):
+            if family == "mixer" and cls.cache_need(part_spec).kind == "paged_kv":
+                if not getattr(cls, "packs_keys_values", False):
+                    raise ConfigError(f"kv_cache 'int4': layers of kind {part_spec.kind!r} keep their cache in the engine's type")
+                if part_spec.head_dim % 32 or part_spec.head_dim > 256:
+                    raise ConfigError(f"kv_cache 'int4': head_dim {part_spec.head_dim} is not a multiple of 32 up to 256")
+                if part_spec.position is not None and part_spec.position.rotary_dim % 8:
+                    raise ConfigError(f"kv_cache 'int4': rotary_dim {part_spec.position.rotary_dim} is not a multiple of 8")
+    return [dataclasses.replace(n, bits=4) if n.kind == "paged_kv" else n for n in needs]
 
 
 def build_part(family: str, part_spec, cls, kernels, dtype, device, name: str = ""):

@@ -8,9 +8,12 @@
     out = (P v) Wo^T (engine/model.py:208).
 The mixer reads whichever cache entry the run order hands it (`call.cache`) and stores its
 own keys and values there only if `call.write` is set, so a layer can read another
-layer's cache.
+layer's cache.  A cache entry may hold its keys and values packed to 4-bit codes (`CacheNeed.bits`
+4, csrc/kv4.cuh): they are then packed as they are stored, and attention reads the codes.
 """
 from __future__ import annotations
+
+import torch
 
 from ..config.specs import CacheNeed
 from ..kernels import materialize
@@ -19,6 +22,7 @@ from .base import ParamSpec, Part
 
 class PagedAttention(Part):
     graph_safe = True
+    packs_keys_values = True             # its cache entry may be a packed one
     prepare_key = "paged_attention"      # every attention layer of a model shares one plan of the step's tiles and items
 
     def __init__(self, spec, kernels, dtype, position):
@@ -78,7 +82,7 @@ class PagedAttention(Part):
             rotated = self.position.encode_and_store(ctx, qkv, view, meta.slots if call.write else None,
                                                      self.heads, self.kv_heads)
             qkv = rotated if rotated is not None else materialize(qkv)
-            self.k.attention(qkv, view, meta, attn, self.heads, self.kv_heads, self.head_dim,
-                             window=self.window, scale=self.scale)
+            attention = self.k.attention_kv4 if view.dtype == torch.uint8 else self.k.attention
+            attention(qkv, view, meta, attn, self.heads, self.kv_heads, self.head_dim, window=self.window, scale=self.scale)
         out = ctx.buffer("attn.out", (t, self.width), self.dtype)
         return self.k.linear(attn, self.o, out, defer=True)

@@ -96,6 +96,9 @@ class RotaryEmbedding(Part):
         return tabs
 
     def encode_and_store(self, ctx, qkv, cache_view, slots, heads, kv_heads):
+        if cache_view.dtype == torch.uint8:            # a packed cache
+            return self.k.rope_store_kv4(qkv, self.tables(ctx) if self.rotary_dim else None, slots, cache_view, heads, kv_heads,
+                                         self.head_dim, self.rotary_dim)
         return self.k.rope_store(qkv, ctx.positions, self.inv_freq, slots, cache_view, heads, kv_heads,
                                  self.head_dim, self.rotary_dim, tables=self.tables(ctx) if self.rotary_dim else None)
 
@@ -112,5 +115,7 @@ class NoPosition(Part):
         self.spec, self.k, self.head_dim = spec, kernels, spec.head_dim
 
     def encode_and_store(self, ctx, qkv, cache_view, slots, heads, kv_heads):
-        if slots is not None:
+        if slots is not None and cache_view.dtype == torch.uint8:
+            self.k.rope_store_kv4(qkv, None, slots, cache_view, heads, kv_heads, self.head_dim, 0)
+        elif slots is not None:
             self.k.rope_store(qkv, ctx.positions, None, slots, cache_view, heads, kv_heads, self.head_dim, 0)

@@ -29,6 +29,7 @@ def parse_args(argv=None):
     ap.add_argument("--page-size", type=int, default=16, help="tokens per cache page")
     ap.add_argument("--max-requests", type=int, default=4, help="state slots: most requests live at a time")
     ap.add_argument("--device", default="cuda:0")
+    ap.add_argument("--kv-cache", default="model", choices=["model", "int4"], help="keys and values in the engine's type, or packed to 4 bits")
     return ap.parse_args(argv)
 
 
@@ -42,7 +43,7 @@ def run(args, lines, out=sys.stdout, kernels=None) -> int:
     pages = max(1, -(-args.max_tokens // args.page_size))
     ec = EngineConfig(dtype=args.dtype, page_size=args.page_size, num_pages=pages, max_num_seqs=args.max_requests,
                       max_num_batched_tokens=max(args.max_tokens, 1), max_model_len=1 << 30, device=args.device,
-                      cuda_graphs=False)
+                      cuda_graphs=False, kv_cache=getattr(args, "kv_cache", "model"))
     engine = build_engine(args.model, ec, kernels=kernels)
     runner, cache = engine.runner, engine.cache
     for line in lines:
