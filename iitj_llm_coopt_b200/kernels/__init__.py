@@ -50,6 +50,12 @@ _SIGNATURES = {
     "llm_kv4_read": [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p],
     "llm_attention_kv4_general": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
                                   _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p],
+    "llm_attention_kv4_single_supported": [_c_int, _c_int, _c_int, _c_int],
+    "llm_attention_kv4_single_tile": [],
+    "llm_attention_kv4_single_warps": [],
+    "llm_attention_kv4_single_resident": [],
+    "llm_attention_kv4_single": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                                 _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p],
     "llm_copy_pages": [_c_void_p, _c_int, ctypes.c_longlong, ctypes.c_longlong, ctypes.POINTER(_c_int), _c_int, _c_void_p],
     "llm_silu_mul": [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p],
     "llm_scale_f32": [_c_void_p, _c_float, ctypes.c_longlong, _c_void_p],
@@ -894,11 +900,56 @@ class Kernels:
               "attention_kv4: one token_request and one position per token")
         if not scale:
             scale = 1.0 / math.sqrt(head_dim)
-        if tokens:
+        if not tokens:
+            return out
+        plan = None
+        if q.dtype == torch.bfloat16 and getattr(meta, "query_lens", None) is not None and q.data_ptr() % 16 == 0 and q.shape[1] % 8 == 0:
+            plan = attention_plan(meta, q.device)
+        if plan is not None and plan.n_tiles == 0 and self.lib.llm_attention_kv4_single_supported(heads, kv_heads, head_dim, page_size):
+            self._kv4_single(q, cache_layer, meta, plan, out, heads, kv_heads, head_dim, page_size, int(window), float(scale))
+        else:
             self._call("llm_attention_kv4_general", _ptr(q), q.shape[1], _ptr(cache_layer), _ptr(meta.block_table), meta.block_table.shape[1],
                        _ptr(meta.token_request), _ptr(meta.positions), _ptr(out), out.shape[1], DTYPE_CODE[q.dtype], tokens, heads, kv_heads,
                        head_dim, page_size, int(window), float(scale), self._stream())
         return out
+
+    def kv4_splits(self, plan, heads, kv_heads, window) -> tuple:
+        """(tiles of 32 keys a block takes, most blocks of any item and head) of a step's single tokens over a packed cache."""
+        key = ("kv4", heads, kv_heads, window, plan.context_bound)
+        if key not in plan._splits:
+            tile, warps = self.lib.llm_attention_kv4_single_tile(), self.lib.llm_attention_kv4_single_warps()
+            slots = self.sm_count * self.lib.llm_attention_kv4_single_resident()
+            grown = max(0, (plan.context_bound or 0) - max(plan.decode_pos) - 1)
+            pos = np.asarray(plan.decode_pos, dtype=np.int64) + grown
+            first = np.maximum(pos - window + 1, 0) if window > 0 else np.zeros_like(pos)
+            spans = pos // tile - first // tile + 1
+            pairs, longest = kv_heads * -(-(heads // kv_heads) // 8), int(spans.max())
+            best = None
+            for n in range(1, max(1, -(-longest // warps)) + 1):
+                per = -(-longest // (n * warps)) * warps
+                blocks = int((-(-spans // per)).sum()) * pairs
+                cost = -(-blocks // slots) * (self.KV4_BLOCK + per // warps) + (self.KV4_JOIN if longest > per else 0.0)
+                if best is None or cost < best[0]:
+                    best = (cost, per)
+                if blocks > 4 * slots:
+                    break
+            plan._splits[key] = (best[1], -(-longest // best[1]))
+        return plan._splits[key]
+
+    # Costs of `kv4_splits`, in the time that a block's warps take for a tile each: a block's start and end, the second kernel.
+    KV4_BLOCK, KV4_JOIN = 2.5, 3.0
+
+    def _kv4_single(self, q, cache_layer, meta, plan, out, heads, kv_heads, head_dim, page_size, window, scale):
+        tiles, splits = self.kv4_splits(plan, heads, kv_heads, window)
+        part_o = part_ml = None
+        if splits > 1:
+            # allocated for the call, not kept: steps on two streams, or of two captured graphs, do not share it
+            part_o = torch.empty(plan.n_items * heads * splits * head_dim, dtype=torch.float32, device=q.device)
+            part_ml = torch.empty(plan.n_items * heads * splits * 2, dtype=torch.float32, device=q.device)
+            self.launches += 1
+        self._call("llm_attention_kv4_single", _ptr(q), q.shape[1], _ptr(cache_layer), _ptr(meta.block_table), meta.block_table.shape[1],
+                   _ptr(plan.items), plan.n_items, _ptr(meta.token_request), _ptr(meta.positions), _ptr(part_o), _ptr(part_ml), _ptr(out),
+                   out.shape[1], heads, kv_heads, head_dim, page_size, window, scale, tiles, splits, self._stream())
 
     def _attention_f32_takes(self, qkv, cache_layer, meta, out, heads, kv_heads, head_dim) -> bool:
         """True if float32 attention runs on the tile and single-token kernels: head sizes 64 and 128, rows on 16-byte

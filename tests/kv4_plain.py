@@ -71,21 +71,18 @@ def store(cache, slots, keys, values, page):
     bad = ~(torch.isfinite(keys.float()).all(-1) & torch.isfinite(values.float()).all(-1) & torch.isfinite(ks).all(-1) &
             torch.isfinite(kz).all(-1) & torch.isfinite(vs).all(-1) & torch.isfinite(vz).all(-1))          # [n, kv]
     regions = _views(cache, kv, page, D)
-    for i, slot in enumerate(slots.tolist()):
-        if slot < 0:
-            continue
-        p, o = divmod(slot, page)
-        for codes, s, z, place, code_region, par_region, is_key in ((kc, ks, kz, key_place, regions[0], regions[1], True),
-                                                                    (vc, vs, vz, value_place, regions[2], regions[3], False)):
-            row = torch.zeros(kv, D // 2, dtype=torch.int32)
-            for c in range(D):
-                byte, shift = place(D, c)
-                row[:, byte] |= codes[i, :, c] << shift
-            par = torch.stack([s[i], z[i]], dim=-1)
-            row[bad[i]] = 0
-            par[bad[i]] = math.nan if is_key else 0.0
-            code_region[p, :, o] = row.to(torch.uint8)
-            par_region[p, :, o] = par.bfloat16().flatten(-2).contiguous().view(torch.uint8)
+    kept = slots >= 0
+    at, off = slots[kept].long() // page, slots[kept].long() % page
+    for codes, s, z, place, which in ((kc, ks, kz, key_place, 0), (vc, vs, vz, value_place, 1)):
+        row = torch.zeros(n, kv, D // 2, dtype=torch.int32)
+        for shift in (0, 4):                       # every byte holds one number at either shift
+            numbers_of = [c for c in range(D) if place(D, c)[1] == shift]
+            row[..., [place(D, c)[0] for c in numbers_of]] |= codes[..., numbers_of] << shift
+        par = torch.stack([s, z], dim=-1)
+        row[bad] = 0
+        par[bad] = math.nan if which == 0 else 0.0
+        regions[2 * which][at, :, off] = row[kept].to(torch.uint8)
+        regions[2 * which + 1][at, :, off] = par.bfloat16().flatten(-2).contiguous().view(torch.uint8)[kept]
 
 
 def numbers(cache, slots, kv, page, D):
@@ -97,11 +94,10 @@ def numbers(cache, slots, kv, page, D):
     for which, place in ((0, key_place), (1, value_place)):
         codes = regions[2 * which][slots // page, :, slots % page]
         par = regions[2 * which + 1][slots // page, :, slots % page].contiguous().view(torch.bfloat16).double().unflatten(-1, (-1, 2))
-        for c in range(D):
-            byte, shift = place(D, c)
-            n = (codes[..., byte].int() >> shift) & 15
-            out_sn[:, which, :, c] = par[..., c // 32, 0] * n
-            out_z[:, which, :, c] = par[..., c // 32, 1]
+        places = [place(D, c) for c in range(D)]
+        n = (codes[..., [p[0] for p in places]].int() >> torch.tensor([p[1] for p in places], dtype=torch.int32)) & 15
+        par = par.repeat_interleave(32, dim=-2)
+        out_sn[:, which], out_z[:, which] = par[..., 0] * n, par[..., 1]
     return out_z, out_sn
 
 

@@ -240,6 +240,21 @@ def test_a_token_that_is_not_finite_reaches_only_those_who_see_it(K, dtype, new)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 130])
+def test_a_query_head_that_is_not_finite_spoils_no_other(K, dtype, new):
+    heads, kv, D, page = 8, 2, 128, 16
+    q, cache, table, meta = case(13, [500], [new], heads, kv, D, page, dtype)
+    clean, got = (torch.empty(new, heads * D, dtype=dtype, device="cuda") for _ in range(2))
+    K.attention_kv4(q.cuda(), cache.cuda(), meta, clean, heads, kv, D)
+    q[0, 2 * D + 5], q[0, 4 * D + 6] = math.nan, math.inf
+    K.attention_kv4(q.cuda(), cache.cuda(), meta, got, heads, kv, D)
+    spoiled = torch.zeros(new, heads, D, dtype=torch.bool)
+    spoiled[0, [2, 4]] = True
+    spoiled = spoiled.flatten(1)
+    assert bool(got.cpu()[spoiled].isnan().all()) and torch.equal(got.cpu()[~spoiled], clean.cpu()[~spoiled])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_a_request_gives_the_same_numbers_in_any_company(K, dtype):
     """The second time, on another stream, captured and replayed: the same bits."""
     heads, kv, D, page = 8, 2, 128, 16
