@@ -23,8 +23,13 @@
 // Replaces flash_attn_varlen_func (engine/model.py:204-207) for portions; same masking and float32
 // statistics as the mma.sync kernel of attention_bf16.cu, which remains for page sizes that do not divide 128.
 //
+// The same kernel over a packed cache (kv4.cuh; any page size that is a multiple of 4): four more warps take the codes apart and write the
+// tiles that TMA would have brought, the cache's numbers z + s n rounded to bfloat16 (one multiply-and-add).  Both heads of a CTA use
+// them, and the work hides beside the softmax, which leaves two thirds of the issue slots free.
+//
 // Every mbarrier wait is bounded; a wait that runs out records a code (llm_attention_tcgen05_status)
 // and the CTA falls through to its teardown, where the tensor memory is freed.
+#include "kv4.cuh"
 #include "tcgen05_common.cuh"
 
 #include <cstdlib>
@@ -38,7 +43,9 @@ constexpr int kRows = 128;        // queries per CTA and head (UMMA M)
 constexpr int kKeys = 128;        // keys per tile
 constexpr int kHalfBytes = 128 * 128;          // 64 dims of 128 rows (queries or keys) as bf16: 128 rows x 128 bytes
 template <int D> __host__ __device__ constexpr int tile_bytes() { return (D / 64) * kHalfBytes; }   // a [128 x D] tile: 16 or 32 KiB
-constexpr int kThreads = 320;     // warp 0: loads, warp 1: MMA + TMEM, warps 2-5: softmax of head A, warps 6-9: of head B
+// warp 0: loads, warp 1: MMA + TMEM, warps 2-5: softmax of head A, warps 6-9: of head B; packed: warps 10-13 unpack
+constexpr int kUnpackWarps = 4, kFirstUnpack = 10;
+template <bool PACKED> __host__ __device__ constexpr int threads() { return PACKED ? 320 + 32 * kUnpackWarps : 320; }
 constexpr int kGroupThreads = 128;
 constexpr uint32_t kTmemCols = 512;            // S_A | S_B | O_A | O_B, 128 float32 columns each (O uses the head's dims)
 #ifndef LLM_ATTN_V_STAGES
@@ -174,6 +181,21 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], uint32_t (&pa
     }
 }
 
+// The eight numbers of a code word (kv4.cuh, key row), z + s n rounded to bfloat16.
+__device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t par) {
+    const uint32_t s2 = __byte_perm(par, par, 0x1010), z2 = __byte_perm(par, par, 0x3232);
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t x;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w >> (4 * i)), "n"(0x000f000f), "r"(0x43004300u));      // 128 + n, exact
+        const __nv_bfloat162 n = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(128.f));
+        const __nv_bfloat162 v = __hfma2(n, *reinterpret_cast<const __nv_bfloat162*>(&s2), *reinterpret_cast<const __nv_bfloat162*>(&z2));
+        r[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
 struct AttnArgs {
     const int* block_table;
     int table_width;
@@ -187,11 +209,12 @@ struct AttnArgs {
     int per_cta;                  // query heads per CTA: 2 (ping-pong), or 1 when that fills more of the GPU
     int pairs;                    // CTAs per key/value group: ceil(heads per group / per_cta)
     float sl;                     // softmax scale * log2(e)
+    const uint8_t* packed;        // the packed cache layer
     int one_pass;                 // tiles after a request's first: one softmax pass (see the kernel); 0: always two (IITJ_ATTN_ONE_PASS=0)
 };
 
-template <int D>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int D, bool PACKED>
+__global__ void __launch_bounds__(threads<PACKED>(), 1)
 attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
                             const AttnArgs a) {
     extern __shared__ unsigned char smem_raw[];
@@ -237,10 +260,10 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1);
+            mbar_init(&k_full[s], PACKED ? kUnpackWarps : 1); mbar_init(&k_empty[s], 1);
             mbar_init(&s_full[s], 1); mbar_init(&p_full[s], kGroupThreads / 32); mbar_init(&o_done[s], 1);
         }
-        for (int s = 0; s < kVStages; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+        for (int s = 0; s < kVStages; ++s) { mbar_init(&v_full[s], PACKED ? kUnpackWarps : 1); mbar_init(&v_empty[s], 1); }
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -269,8 +292,8 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const int* table = a.block_table + (size_t)req * a.table_width;
         const int ps = a.page_size, pages_per_tile = kKeys / ps;
         int page = 0;
-        if (lane < pages_per_tile) page = table[min(k_begin / ps + lane, a.table_width - 1)];
-        for (int j = 0; j < n_tiles; ++j) {
+        if (!PACKED && lane < pages_per_tile) page = table[min(k_begin / ps + lane, a.table_width - 1)];
+        for (int j = 0; j < (PACKED ? 0 : n_tiles); ++j) {
             const int s = j & 1, sv = j % kVStages;
             int ok = 1;
             if (lane == 0) {
@@ -356,6 +379,76 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             }
             umma_commit(&v_empty[j % kVStages]);
             if (more) umma_commit(&k_empty[s1]);
+        }
+    } else if (PACKED && warp >= kFirstUnpack) {
+        // ---- unpacking: warp p takes the octets p, p + 4, ... of a tile's 128 keys ------------------------------------------------
+        // Lane 8 j + r reads 4 G bytes of codes of key r of an octet, which are numbers 8 j .. 8 j + 7 of every group, and writes them as
+        // G chunks of 16 bytes; eight lanes of one j write to all banks.  A value row's two half-words of eight numbers make such a word too.
+        constexpr int G = D / 32, kOctets = kKeys / 8 / kUnpackWarps;
+        const int p = warp - kFirstUnpack, jj = lane >> 3, r = lane & 7;
+        const int* table = a.block_table + (size_t)req * a.table_width;
+        const int ps = a.page_size;
+        const size_t block_bytes = kv4_block_bytes(ps, G);
+        const uint8_t* cache = a.packed + (size_t)hk * block_bytes;
+        const size_t page_bytes = (size_t)a.kv_heads * block_bytes;
+        struct Units { uint32_t w[kOctets][G], par[kOctets][G]; };
+        // Lane x looks up the page of keys 4 x .. 4 x + 3 of a tile (they share one).  Keys outside the rows' reach are taken from its ends:
+        // nothing behind a request's last token, or in a page given back, is read.
+        auto look_up = [&](int j, int& quad, int& page) {
+            quad = min(max(k_begin + j * kKeys + 4 * lane, lo0 & ~3), pos_last & ~3);
+            page = table[quad / ps];
+        };
+        auto fetch = [&](Units& u, int quad, int page, int region) {          // region: 0 keys, 1 values
+#pragma unroll
+            for (int i = 0; i < kOctets; ++i) {
+                const int from = 2 * (p + kUnpackWarps * i) + (r >> 2);
+                const int q0 = __shfl_sync(0xffffffffu, quad, from), pg = __shfl_sync(0xffffffffu, page, from);
+                const int off = min(max(q0 + (r & 3), lo0), pos_last) % ps;
+                const uint8_t* at = cache + (size_t)pg * page_bytes + (size_t)region * ps * 20 * G;
+                const uint8_t *codes = at + off * 16 * G + 4 * G * jj, *par = at + ps * 16 * G + off * 4 * G;
+                if constexpr (G == 4) {
+                    const uint4 c = *reinterpret_cast<const uint4*>(codes), q = *reinterpret_cast<const uint4*>(par);
+                    u.w[i][0] = c.x; u.w[i][1] = c.y; u.w[i][2] = c.z; u.w[i][3] = c.w;
+                    u.par[i][0] = q.x; u.par[i][1] = q.y; u.par[i][2] = q.z; u.par[i][3] = q.w;
+                } else {
+                    const uint2 c = *reinterpret_cast<const uint2*>(codes), q = *reinterpret_cast<const uint2*>(par);
+                    u.w[i][0] = c.x; u.w[i][1] = c.y;
+                    u.par[i][0] = q.x; u.par[i][1] = q.y;
+                }
+            }
+        };
+        auto write = [&](const Units& u, unsigned char* tile, bool value) {
+#pragma unroll
+            for (int i = 0; i < kOctets; ++i) {
+                unsigned char* row = tile + (p + kUnpackWarps * i) * 1024 + r * 128;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const uint32_t w = value ? __byte_perm(u.w[i][g / 2], u.w[i][G / 2 + g / 2], (g & 1) ? 0x7632 : 0x5410) : u.w[i][g];
+                    const int chunk = 4 * g + jj;
+                    *reinterpret_cast<uint4*>(row + (chunk >> 3) * kHalfBytes + (((chunk & 7) ^ r) << 4)) = unpack_word(w, u.par[i][g]);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the tensor core reads these through the async proxy
+            __syncwarp();
+        };
+        Units keys, values;
+        int quad, page, quad_next, page_next;
+        look_up(0, quad, page);
+        fetch(keys, quad, page, 0);
+        for (int j = 0; j < n_tiles; ++j) {
+            const int s = j & 1, sv = j % kVStages;
+            fetch(values, quad, page, 1);
+            if (j + 1 < n_tiles) look_up(j + 1, quad_next, page_next);
+            if (j >= 2 && !mbar_wait_all(&k_empty[s], ((j >> 1) - 1) & 1)) { attn_give_up(1); failed = 1; break; }
+            write(keys, k_tile[s], false);
+            if (lane == 0) mbar_arrive(&k_full[s]);
+            if (j + 1 < n_tiles) {
+                quad = quad_next; page = page_next;
+                fetch(keys, quad, page, 0);
+            }
+            if (j >= kVStages && !mbar_wait_all(&v_empty[sv], ((j / kVStages) - 1) & 1)) { attn_give_up(1); failed = 1; break; }
+            write(values, v_tile[sv], true);
+            if (lane == 0) mbar_arrive(&v_full[sv]);
         }
     } else if (warp >= 2 && ((warp - 2) >> 2) < n_heads) {
         // ---- softmax and output: one thread per query row of one head ---------------------------------
@@ -612,25 +705,25 @@ LLM_API int llm_attention_tcgen05_supported(int heads, int kv_heads, int head_di
            (128 % page_size) == 0;
 }
 
-// q: [tokens, q_stride] bf16 with head h at columns [h * head_dim, (h + 1) * head_dim); cache layer [pages, 2, kv_heads, page, head_dim];
-// tiles: [n_tiles] int4 {first token row, rows (<= 128), position of the first row, request}.
-LLM_API int llm_attention_prefill_tcgen05(const void* q, int q_stride, int tokens, const void* cache, long long cache_pages,
-                                          const int* block_table, int table_width, const int* tiles, int n_tiles,
-                                          void* out, int out_stride, int heads, int kv_heads, int head_dim,
-                                          int page_size, int window, float scale, int splits, float* part_o,
-                                          float* part_ml, cudaStream_t stream) {
-    if (n_tiles == 0) return 0;
-    if (!llm_attention_tcgen05_supported(heads, kv_heads, head_dim, page_size))
-        LLM_FAIL(-1, "attention_prefill_tcgen05: heads %d / kv_heads %d / head_dim %d / page %d not supported", heads,
-                 kv_heads, head_dim, page_size);
+namespace {
+
+template <bool PACKED>
+int launch_prefill(const void* q, int q_stride, int tokens, const void* cache, long long cache_pages, const int* block_table,
+                   int table_width, const int* tiles, int n_tiles, void* out, int out_stride, int heads, int kv_heads, int head_dim,
+                   int page_size, int window, float scale, int splits, float* part_o, float* part_ml, cudaStream_t stream) {
     if (heads > 65535) LLM_FAIL(-1, "attention_prefill_tcgen05: too many heads");
     if (out_stride % 8) LLM_FAIL(-1, "attention_prefill_tcgen05: out_stride must be a multiple of 8");
     CUtensorMap mq, mkv;
     if (int rc = llm_tensor_map_2d(q, (uint64_t)tokens, (uint64_t)q_stride, kRows, 64, &mq)) return rc;
-    const uint64_t kv_rows = (uint64_t)cache_pages * 2 * kv_heads * page_size;
-    if (kv_rows > 0x7fffffffull) LLM_FAIL(-1, "attention_prefill_tcgen05: the cache layer has too many rows for 32-bit TMA coordinates");
-    if (int rc = llm_tensor_map_2d(cache, kv_rows, (uint64_t)head_dim, (uint32_t)page_size, 64, &mkv)) return rc;
+    if (PACKED) {
+        mkv = mq;                 // (the packed cache is read without a map)
+    } else {
+        const uint64_t kv_rows = (uint64_t)cache_pages * 2 * kv_heads * page_size;
+        if (kv_rows > 0x7fffffffull) LLM_FAIL(-1, "attention_prefill_tcgen05: the cache layer has too many rows for 32-bit TMA coordinates");
+        if (int rc = llm_tensor_map_2d(cache, kv_rows, (uint64_t)head_dim, (uint32_t)page_size, 64, &mkv)) return rc;
+    }
     AttnArgs a;
+    a.packed = PACKED ? (const uint8_t*)cache : nullptr;
     a.block_table = block_table;
     a.table_width = table_width;
     a.tiles = (const int4*)tiles;
@@ -656,10 +749,10 @@ LLM_API int llm_attention_prefill_tcgen05(const void* q, int q_stride, int token
     const size_t smem = (4 + kVStages) * (size_t)(head_dim == 64 ? tile_bytes<64>() : tile_bytes<128>()) + 1024;
     static bool configured = false;
     if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(attn_prefill_tcgen05_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        cudaError_t e = cudaFuncSetAttribute(attn_prefill_tcgen05_kernel<128, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (4 + kVStages) * tile_bytes<128>() + 1024);
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(attn_prefill_tcgen05_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            e = cudaFuncSetAttribute(attn_prefill_tcgen05_kernel<64, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (4 + kVStages) * tile_bytes<64>() + 1024);
         if (e != cudaSuccess) LLM_FAIL(-2, "attention_prefill_tcgen05: %s", cudaGetErrorString(e));
         configured = true;
@@ -670,8 +763,8 @@ LLM_API int llm_attention_prefill_tcgen05(const void* q, int q_stride, int token
     a.part_o = part_o;
     a.part_ml = part_ml;
     const dim3 grid(n_tiles, kv_heads * a.pairs, splits), merge_grid(n_tiles * (kRows / (kMergeThreads / (head_dim / 4))), heads);
-    if (head_dim == 64) llm_launch(attn_prefill_tcgen05_kernel<64>, grid, kThreads, smem, stream, mq, mkv, a);
-    else llm_launch(attn_prefill_tcgen05_kernel<128>, grid, kThreads, smem, stream, mq, mkv, a);
+    if (head_dim == 64) llm_launch(attn_prefill_tcgen05_kernel<64, PACKED>, grid, threads<PACKED>(), smem, stream, mq, mkv, a);
+    else llm_launch(attn_prefill_tcgen05_kernel<128, PACKED>, grid, threads<PACKED>(), smem, stream, mq, mkv, a);
     LLM_CHECK_LAUNCH("attention_prefill_tcgen05");
     if (splits > 1) {
         auto merge = [&](auto small, auto middle, auto large) {
@@ -682,6 +775,39 @@ LLM_API int llm_attention_prefill_tcgen05(const void* q, int q_stride, int token
         LLM_CHECK_LAUNCH("attention_prefill_tcgen05 merge");
     }
     return 0;
+}
+
+}  // namespace
+
+// q: [tokens, q_stride] bf16 with head h at columns [h * head_dim, (h + 1) * head_dim); cache layer [pages, 2, kv_heads, page, head_dim];
+// tiles: [n_tiles] int4 {first token row, rows (<= 128), position of the first row, request}.
+LLM_API int llm_attention_prefill_tcgen05(const void* q, int q_stride, int tokens, const void* cache, long long cache_pages,
+                                          const int* block_table, int table_width, const int* tiles, int n_tiles,
+                                          void* out, int out_stride, int heads, int kv_heads, int head_dim,
+                                          int page_size, int window, float scale, int splits, float* part_o,
+                                          float* part_ml, cudaStream_t stream) {
+    if (n_tiles == 0) return 0;
+    if (!llm_attention_tcgen05_supported(heads, kv_heads, head_dim, page_size))
+        LLM_FAIL(-1, "attention_prefill_tcgen05: heads %d / kv_heads %d / head_dim %d / page %d not supported", heads,
+                 kv_heads, head_dim, page_size);
+    return launch_prefill<false>(q, q_stride, tokens, cache, cache_pages, block_table, table_width, tiles, n_tiles, out, out_stride, heads,
+                                 kv_heads, head_dim, page_size, window, scale, splits, part_o, part_ml, stream);
+}
+
+// 1 if the kernel over a packed cache takes this geometry.
+LLM_API int llm_attention_kv4_prompt_supported(int heads, int kv_heads, int head_dim, int page_size) {
+    return (head_dim == 64 || head_dim == 128) && kv_heads > 0 && heads % kv_heads == 0 && kv4_geometry(head_dim, page_size);
+}
+
+// The same over a packed cache layer (kv4.cuh).
+LLM_API int llm_attention_kv4_prompt(const void* q, int q_stride, int tokens, const void* cache, const int* block_table, int table_width,
+                                     const int* tiles, int n_tiles, void* out, int out_stride, int heads, int kv_heads, int head_dim,
+                                     int page_size, int window, float scale, int splits, float* part_o, float* part_ml, cudaStream_t stream) {
+    if (n_tiles == 0) return 0;
+    if (!llm_attention_kv4_prompt_supported(heads, kv_heads, head_dim, page_size))
+        LLM_FAIL(-1, "attention_kv4_prompt: heads %d / kv_heads %d / head_dim %d / page %d not supported", heads, kv_heads, head_dim, page_size);
+    return launch_prefill<true>(q, q_stride, tokens, cache, 0, block_table, table_width, tiles, n_tiles, out, out_stride, heads, kv_heads,
+                                head_dim, page_size, window, scale, splits, part_o, part_ml, stream);
 }
 
 const int* llm_attention_tcgen05_status_word() {

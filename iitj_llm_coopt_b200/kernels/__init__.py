@@ -56,6 +56,9 @@ _SIGNATURES = {
     "llm_attention_kv4_single_resident": [],
     "llm_attention_kv4_single": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                  _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p],
+    "llm_attention_kv4_prompt_supported": [_c_int, _c_int, _c_int, _c_int],
+    "llm_attention_kv4_prompt": [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int,
+                                 _c_int, _c_int, _c_int, _c_float, _c_int, _c_void_p, _c_void_p, _c_void_p],
     "llm_copy_pages": [_c_void_p, _c_int, ctypes.c_longlong, ctypes.c_longlong, ctypes.POINTER(_c_int), _c_int, _c_void_p],
     "llm_silu_mul": [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p],
     "llm_scale_f32": [_c_void_p, _c_float, ctypes.c_longlong, _c_void_p],
@@ -905,13 +908,32 @@ class Kernels:
         plan = None
         if q.dtype == torch.bfloat16 and getattr(meta, "query_lens", None) is not None and q.data_ptr() % 16 == 0 and q.shape[1] % 8 == 0:
             plan = attention_plan(meta, q.device)
-        if plan is not None and plan.n_tiles == 0 and self.lib.llm_attention_kv4_single_supported(heads, kv_heads, head_dim, page_size):
-            self._kv4_single(q, cache_layer, meta, plan, out, heads, kv_heads, head_dim, page_size, int(window), float(scale))
+        shape = (heads, kv_heads, head_dim, page_size)
+        if plan is not None and (not plan.n_tiles or self.lib.llm_attention_kv4_prompt_supported(*shape)) and \
+                (not plan.n_items or self.lib.llm_attention_kv4_single_supported(*shape)):
+            if plan.n_tiles:
+                self._kv4_prompt(q, cache_layer, meta, plan, out, *shape, int(window), float(scale))
+            if plan.n_items:
+                self._kv4_single(q, cache_layer, meta, plan, out, *shape, int(window), float(scale))
         else:
             self._call("llm_attention_kv4_general", _ptr(q), q.shape[1], _ptr(cache_layer), _ptr(meta.block_table), meta.block_table.shape[1],
                        _ptr(meta.token_request), _ptr(meta.positions), _ptr(out), out.shape[1], DTYPE_CODE[q.dtype], tokens, heads, kv_heads,
                        head_dim, page_size, int(window), float(scale), self._stream())
         return out
+
+    def _kv4_prompt(self, q, cache_layer, meta, plan, out, heads, kv_heads, head_dim, page_size, window, scale):
+        if plan.big_tiles is None:
+            plan.big_tiles = torch.tensor(plan.big_rows, dtype=torch.int32).to(q.device)
+        splits = self.prefill_key_splits(plan.big_rows, heads, kv_heads, window)
+        part_o = part_ml = None
+        if splits > 1:       # (allocated for the call, as in _kv4_single)
+            n = len(plan.big_rows) * heads * splits * 128
+            part_o = torch.empty(n * head_dim, dtype=torch.float32, device=q.device)
+            part_ml = torch.empty(n * 2, dtype=torch.float32, device=q.device)
+            self.launches += 1
+        self._call("llm_attention_kv4_prompt", _ptr(q), q.shape[1], q.shape[0], _ptr(cache_layer), _ptr(meta.block_table),
+                   meta.block_table.shape[1], _ptr(plan.big_tiles), len(plan.big_rows), _ptr(out), out.shape[1], heads, kv_heads, head_dim,
+                   page_size, window, scale, splits, _ptr(part_o), _ptr(part_ml), self._stream())
 
     def kv4_splits(self, plan, heads, kv_heads, window) -> tuple:
         """(tiles of 32 keys a block takes, most blocks of any item and head) of a step's single tokens over a packed cache."""

@@ -244,6 +244,7 @@ def test_a_token_that_is_not_finite_reaches_only_those_who_see_it(K, dtype, new)
 def test_a_query_head_that_is_not_finite_spoils_no_other(K, dtype, new):
     heads, kv, D, page = 8, 2, 128, 16
     q, cache, table, meta = case(13, [500], [new], heads, kv, D, page, dtype)
+    want, tol = P.attend(q, cache, table, [500], [new], heads, kv, page, D, unit=P.U16 if dtype == torch.bfloat16 else P.U32)
     clean, got = (torch.empty(new, heads * D, dtype=dtype, device="cuda") for _ in range(2))
     K.attention_kv4(q.cuda(), cache.cuda(), meta, clean, heads, kv, D)
     q[0, 2 * D + 5], q[0, 4 * D + 6] = math.nan, math.inf
@@ -251,7 +252,10 @@ def test_a_query_head_that_is_not_finite_spoils_no_other(K, dtype, new):
     spoiled = torch.zeros(new, heads, D, dtype=torch.bool)
     spoiled[0, [2, 4]] = True
     spoiled = spoiled.flatten(1)
-    assert bool(got.cpu()[spoiled].isnan().all()) and torch.equal(got.cpu()[~spoiled], clean.cpu()[~spoiled])
+    assert bool(got.cpu()[spoiled].isnan().all())
+    # (heads that share a warp share the decision to move the reference of their sums: the others' last bits may differ)
+    for x in (got, clean):
+        assert bool(((x.cpu().double() - want).abs() <= tol)[~spoiled].all())
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
