@@ -391,21 +391,37 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const size_t block_bytes = kv4_block_bytes(ps, G);
         const uint8_t* cache = a.packed + (size_t)hk * block_bytes;
         const size_t page_bytes = (size_t)a.kv_heads * block_bytes;
+        const int page_shift = (ps & (ps - 1)) ? -1 : 31 - __clz(ps), value_at = ps * 20 * G, par_at = ps * 16 * G;
         struct Units { uint32_t w[kOctets][G], par[kOctets][G]; };
-        // Lane x looks up the page of keys 4 x .. 4 x + 3 of a tile (they share one).  Keys outside the rows' reach are taken from its ends:
-        // nothing behind a request's last token, or in a page given back, is read.
-        auto look_up = [&](int j, int& quad, int& page) {
-            quad = min(max(k_begin + j * kKeys + 4 * lane, lo0 & ~3), pos_last & ~3);
-            page = table[quad / ps];
+        struct Rows { const uint8_t* codes[kOctets]; const uint8_t* par[kOctets]; };
+        // Lane x looks up the page of keys 4 x .. 4 x + 3 of a tile (they share one), and the first one's place in it.  Keys outside the
+        // rows' reach are taken from its ends: nothing behind a request's last token, or in a page given back, is read.
+        auto look_up = [&](int j, int& page, int& off) {
+            const int quad = min(max(k_begin + j * kKeys + 4 * lane, lo0 & ~3), pos_last & ~3);
+            const int lp = page_shift >= 0 ? quad >> page_shift : quad / ps;
+            page = table[lp];
+            off = quad - lp * ps;
         };
-        auto fetch = [&](Units& u, int quad, int page, int region) {          // region: 0 keys, 1 values
+        auto find = [&](Rows& rows, int j, int page, int off) {               // the key rows of this lane's octets
+            const int k0 = k_begin + j * kKeys;
+            const bool edge = k0 < lo0 || k0 + kKeys - 1 > pos_last;
 #pragma unroll
             for (int i = 0; i < kOctets; ++i) {
-                const int from = 2 * (p + kUnpackWarps * i) + (r >> 2);
-                const int q0 = __shfl_sync(0xffffffffu, quad, from), pg = __shfl_sync(0xffffffffu, page, from);
-                const int off = min(max(q0 + (r & 3), lo0), pos_last) % ps;
-                const uint8_t* at = cache + (size_t)pg * page_bytes + (size_t)region * ps * 20 * G;
-                const uint8_t *codes = at + off * 16 * G + 4 * G * jj, *par = at + ps * 16 * G + off * 4 * G;
+                const int octet = p + kUnpackWarps * i, from = 2 * octet + (r >> 2);
+                int at = __shfl_sync(0xffffffffu, off, from) + (r & 3);
+                if (edge) {
+                    const int quad = min(max(k0 + 4 * from, lo0 & ~3), pos_last & ~3);
+                    at += min(max(quad + (r & 3), lo0), pos_last) - (quad + (r & 3));
+                }
+                const uint8_t* page_at = cache + (size_t)__shfl_sync(0xffffffffu, page, from) * page_bytes;
+                rows.codes[i] = page_at + at * 16 * G + 4 * G * jj;
+                rows.par[i] = page_at + par_at + at * 4 * G;
+            }
+        };
+        auto fetch = [&](Units& u, const Rows& rows, int region) {            // region: 0, or value_at
+#pragma unroll
+            for (int i = 0; i < kOctets; ++i) {
+                const uint8_t *codes = rows.codes[i] + region, *par = rows.par[i] + region;
                 if constexpr (G == 4) {
                     const uint4 c = *reinterpret_cast<const uint4*>(codes), q = *reinterpret_cast<const uint4*>(par);
                     u.w[i][0] = c.x; u.w[i][1] = c.y; u.w[i][2] = c.z; u.w[i][3] = c.w;
@@ -432,19 +448,21 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             __syncwarp();
         };
         Units keys, values;
-        int quad, page, quad_next, page_next;
-        look_up(0, quad, page);
-        fetch(keys, quad, page, 0);
+        Rows rows;
+        int page, off;
+        look_up(0, page, off);
+        find(rows, 0, page, off);
+        fetch(keys, rows, 0);
         for (int j = 0; j < n_tiles; ++j) {
             const int s = j & 1, sv = j % kVStages;
-            fetch(values, quad, page, 1);
-            if (j + 1 < n_tiles) look_up(j + 1, quad_next, page_next);
+            fetch(values, rows, value_at);
+            if (j + 1 < n_tiles) look_up(j + 1, page, off);
             if (j >= 2 && !mbar_wait_all(&k_empty[s], ((j >> 1) - 1) & 1)) { attn_give_up(1); failed = 1; break; }
             write(keys, k_tile[s], false);
             if (lane == 0) mbar_arrive(&k_full[s]);
             if (j + 1 < n_tiles) {
-                quad = quad_next; page = page_next;
-                fetch(keys, quad, page, 0);
+                find(rows, j + 1, page, off);
+                fetch(keys, rows, 0);
             }
             if (j >= kVStages && !mbar_wait_all(&v_empty[sv], ((j / kVStages) - 1) & 1)) { attn_give_up(1); failed = 1; break; }
             write(values, v_tile[sv], true);
