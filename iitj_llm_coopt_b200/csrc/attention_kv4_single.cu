@@ -493,7 +493,15 @@ LLM_API int llm_attention_kv4_single(const void* q, int q_stride, const void* ca
     if ((long long)kv_heads * a.head_tiles > 65535 || n_items > 65535) LLM_FAIL(-1, "attention_kv4_single: too many heads or items");
     const dim3 grid(max_splits, kv_heads * a.head_tiles, n_items);
     auto go = [&](auto kernel, auto join, size_t smem) -> int {
-        LLM_ALLOW_SMEM("attention_kv4_single", kernel, smem);
+        // (asked for once a device: the driver's call takes longer than the launch)
+        static unsigned long long allowed[2] = {0, 0};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        unsigned long long& done = allowed[head_dim == 64];
+        if (dev >= 64 || !(done >> dev & 1)) {
+            LLM_ALLOW_SMEM("attention_kv4_single", kernel, smem);
+            if (dev < 64) done |= 1ull << dev;
+        }
         llm_launch(kernel, grid, kWarps * 32, smem, stream, a);
         LLM_CHECK_LAUNCH("attention_kv4_single");
         if (max_splits > 1) {

@@ -9,6 +9,9 @@
 // their wait for the kernel before them, which must not reach past a copy of such keys.
 #include "common.cuh"
 
+#include <algorithm>
+#include <cstdlib>
+
 namespace {
 
 constexpr int kMaxPairs = 256;                 // pairs a launch carries (2 KB of parameters)
@@ -43,7 +46,19 @@ LLM_API int llm_copy_pages(void* pool, int entries, long long pages, long long p
     if (n_pairs == 0 || entries == 0 || page_bytes == 0) return 0;
     if (entries < 0 || entries > 65535) LLM_FAIL(-1, "copy_pages: %d entries (at most 65535)", entries);
     for (int i = 0; i < 2 * n_pairs; ++i)
-        if (pairs[i] < 0 || pairs[i] >= pages) LLM_FAIL(-1, "copy_pages: page %d is not one of the pool's %lld", pairs[i], pages);
+        if (pairs[i] < 0 || pairs[i] >= pages) LLM_FAIL(-1, "copy_pages: page %d is not one of the pool's %lld pages", pairs[i], pages);
+    // no destination twice, none that is a source: pages by what they are, side by side once sorted (2 page: source, + 1: destination)
+    long long few[512];
+    long long* seen = 2 * n_pairs <= 512 ? few : static_cast<long long*>(malloc(2 * (size_t)n_pairs * sizeof(long long)));
+    if (!seen) LLM_FAIL(-2, "copy_pages: no memory for %d pairs", n_pairs);
+    for (int i = 0; i < 2 * n_pairs; ++i) seen[i] = 2ll * pairs[i] + (i & 1);
+    std::sort(seen, seen + 2 * n_pairs);
+    int clash = -1, twice = 0;
+    for (int i = 1; i < 2 * n_pairs && clash < 0; ++i)
+        if (seen[i] / 2 == seen[i - 1] / 2 && (seen[i] & 1)) { clash = (int)(seen[i] / 2); twice = (int)(seen[i - 1] & 1); }
+    if (seen != few) free(seen);
+    if (clash >= 0)
+        LLM_FAIL(-1, twice ? "copy_pages: page %d is the destination of two copies" : "copy_pages: page %d is the source of one copy and the destination of another", clash);
     const unsigned long long low = (unsigned long long)(uintptr_t)pool | (unsigned long long)page_bytes;
     const int width = low % 16 == 0 ? 16 : low % 4 == 0 ? 4 : 1;
     const long long slices = (page_bytes / width + kCopyThreads * kCopyPer - 1) / (kCopyThreads * kCopyPer);

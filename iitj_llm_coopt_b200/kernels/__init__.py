@@ -15,6 +15,7 @@ F.linear); `gemm_policy` holds the measurements behind the choice.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import math
 import os
@@ -59,7 +60,7 @@ _SIGNATURES = {
     "llm_attention_kv4_prompt_supported": [_c_int, _c_int, _c_int, _c_int],
     "llm_attention_kv4_prompt": [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int,
                                  _c_int, _c_int, _c_int, _c_float, _c_int, _c_void_p, _c_void_p, _c_void_p],
-    "llm_copy_pages": [_c_void_p, _c_int, ctypes.c_longlong, ctypes.c_longlong, ctypes.POINTER(_c_int), _c_int, _c_void_p],
+    "llm_copy_pages": [_c_void_p, _c_int, ctypes.c_longlong, ctypes.c_longlong, _c_void_p, _c_int, _c_void_p],
     "llm_silu_mul": [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p],
     "llm_scale_f32": [_c_void_p, _c_float, ctypes.c_longlong, _c_void_p],
     "llm_sum_parts": [_c_void_p, _c_void_p, _c_int, _c_int, ctypes.c_longlong, _c_void_p],
@@ -446,6 +447,8 @@ class Kernels:
             self.lib.llm_set_pdl(0)
         self._scratch_bufs: dict = {}
         self._pair_counters: dict = {}
+        self._kv4_pages: dict = {}       # (bytes of a page, kv_heads, head_dim) -> tokens of a packed page
+        self._kv4_forms: dict = {}       # (heads, kv_heads, head_dim, page size) -> whether the packed prompt and single-token kernels take it
         self._linear_plans: dict = {}    # (tokens, n, k, swiglu) -> (kernel, k-splits, shared memory, half-tile form)
         self.scratch_generation = 0
         self._sm_count = None
@@ -707,16 +710,19 @@ class Kernels:
         return qkv
 
     # ---- packed keys and values, pages of a cache ------------------------------------
-    @staticmethod
-    def _kv4_page_size(name, cache_layer, kv_heads, head_dim) -> int:
+    def _kv4_page_size(self, name, cache_layer, kv_heads, head_dim) -> int:
         """Tokens a page of a packed cache layer [pages, bytes] holds (csrc/kv4.cuh)."""
         _check(cache_layer, name + ".cache", torch.uint8, 2)
-        _need(head_dim % 32 == 0 and 32 <= head_dim <= 256, f"{name}: head_dim {head_dim} is not a multiple of 32 up to 256")
-        token = kv_heads * (head_dim // 32) * 40
-        _need(kv_heads > 0 and cache_layer.shape[1] % (4 * token) == 0 and cache_layer.shape[1] > 0,
-              f"{name}.cache: pages of {cache_layer.shape[1]} bytes are no multiple of 4 tokens of {kv_heads} heads of {head_dim} numbers")
+        key = (cache_layer.shape[1], kv_heads, head_dim)
+        page_size = self._kv4_pages.get(key)
+        if page_size is None:
+            _need(head_dim % 32 == 0 and 32 <= head_dim <= 256, f"{name}: head_dim {head_dim} is not a multiple of 32 up to 256")
+            token = kv_heads * (head_dim // 32) * 40
+            _need(kv_heads > 0 and cache_layer.shape[1] % (4 * token) == 0 and cache_layer.shape[1] > 0,
+                  f"{name}.cache: pages of {cache_layer.shape[1]} bytes are no multiple of 4 tokens of {kv_heads} heads of {head_dim} numbers")
+            page_size = self._kv4_pages[key] = cache_layer.shape[1] // token
         _need(cache_layer.data_ptr() % 16 == 0, f"{name}.cache: not on a 16-byte boundary")
-        return cache_layer.shape[1] // token
+        return page_size
 
     def rope_store_kv4(self, qkv, tables, slots, cache_layer, heads, kv_heads, head_dim, rotary_dim, q_out=None):
         """`rope_store` into a packed cache: rotates the queries, rotates and packs the keys, packs the values and stores both in
@@ -736,7 +742,7 @@ class Kernels:
         tokens = qkv.shape[0]
         _need(heads > 0 and kv_heads > 0 and qkv.shape[1] == (heads + 2 * kv_heads) * head_dim,
               "rope_store_kv4.qkv: width is not (heads+2*kv_heads)*head_dim")
-        _need(0 <= rotary_dim <= head_dim and rotary_dim % 8 == 0, f"rope_store_kv4: rotary_dim {rotary_dim} is not a multiple of 8 up to {head_dim}")
+        _need(0 <= rotary_dim <= head_dim and rotary_dim % 16 == 0, f"rope_store_kv4: rotary_dim {rotary_dim} is not a multiple of 16 up to {head_dim}")
         _need(head_dim % 32 == 0 and 32 <= head_dim <= 256, f"rope_store_kv4: head_dim {head_dim} is not a multiple of 32 up to 256")
         cos = sin = None
         if rotary_dim:
@@ -780,17 +786,14 @@ class Kernels:
         destination may be another pair's destination or anybody's source.  storage: [entries, pages, ...] of any type."""
         _check(storage, "copy_pages.storage")
         _need(storage.dim() >= 2, f"copy_pages.storage: want [entries, pages, ...], got shape {tuple(storage.shape)}")
-        pairs = [(int(a), int(b)) for a, b in pairs]
-        pages = storage.shape[1]
-        for a, b in pairs:
-            _need(0 <= a < pages and 0 <= b < pages, f"copy_pages: ({a}, {b}) are not both among the pool's {pages} pages")
-        targets = {b for _, b in pairs}
-        _need(len(targets) == len(pairs), "copy_pages: a page is the destination of two copies")
-        _need(not targets & {a for a, _ in pairs}, "copy_pages: a page is the source of one copy and the destination of another")
-        if pairs and storage.numel():
-            flat = (_c_int * (2 * len(pairs)))(*(x for pair in pairs for x in pair))
-            self._call("llm_copy_pages", _ptr(storage), storage.shape[0], pages, storage[0, 0].numel() * storage.element_size(), flat,
-                       len(pairs), self._stream())
+        try:
+            flat = array.array("i", [x for src, dst in pairs for x in (src, dst)])
+        except (TypeError, ValueError, OverflowError) as e:
+            raise KernelError(f"copy_pages.pairs: (source, destination) page ids are wanted: {e}") from None
+        if flat and storage.numel():
+            entries, pages = storage.shape[:2]
+            self._call("llm_copy_pages", _ptr(storage), entries, pages, storage.numel() // (entries * pages) * storage.element_size(),
+                       flat.buffer_info()[0], len(pairs), self._stream())
             self.launches += (len(pairs) - 1) // 256          # a launch carries 256 pairs
         return storage
 
@@ -909,8 +912,10 @@ class Kernels:
         if q.dtype == torch.bfloat16 and getattr(meta, "query_lens", None) is not None and q.data_ptr() % 16 == 0 and q.shape[1] % 8 == 0:
             plan = attention_plan(meta, q.device)
         shape = (heads, kv_heads, head_dim, page_size)
-        if plan is not None and (not plan.n_tiles or self.lib.llm_attention_kv4_prompt_supported(*shape)) and \
-                (not plan.n_items or self.lib.llm_attention_kv4_single_supported(*shape)):
+        forms = self._kv4_forms.get(shape)
+        if forms is None:
+            forms = self._kv4_forms[shape] = (self.lib.llm_attention_kv4_prompt_supported(*shape), self.lib.llm_attention_kv4_single_supported(*shape))
+        if plan is not None and (not plan.n_tiles or forms[0]) and (not plan.n_items or forms[1]):
             if plan.n_tiles:
                 self._kv4_prompt(q, cache_layer, meta, plan, out, *shape, int(window), float(scale))
             if plan.n_items:

@@ -104,8 +104,8 @@ def packed_cache_needs(spec, page_size: int) -> list:
                     raise ConfigError(f"kv_cache 'int4': layers of kind {part_spec.kind!r} keep their cache in the engine's type")
                 if part_spec.head_dim % 32 or part_spec.head_dim > 256:
                     raise ConfigError(f"kv_cache 'int4': head_dim {part_spec.head_dim} is not a multiple of 32 up to 256")
-                if part_spec.position is not None and part_spec.position.rotary_dim % 8:
-                    raise ConfigError(f"kv_cache 'int4': rotary_dim {part_spec.position.rotary_dim} is not a multiple of 8")
+                if part_spec.position is not None and part_spec.position.rotary_dim % 16:
+                    raise ConfigError(f"kv_cache 'int4': rotary_dim {part_spec.position.rotary_dim} is not a multiple of 16")
     return [dataclasses.replace(n, bits=4) if n.kind == "paged_kv" else n for n in needs]
 
 

@@ -364,7 +364,8 @@ def test_refusals(K):
             K.attention_kv4(**{**good, **bad})
     pool = z(2, 6, 32)
     for pairs, text in (([(0, 6)], "pool's 6 pages"), ([(-1, 2)], "pool's 6 pages"), ([(0, 1), (2, 1)], "two copies"),
-                        ([(0, 1), (1, 2)], "source of one"), ([(3, 3)], "source of one")):
+                        ([(0, 1), (1, 2)], "source of one"), ([(3, 3)], "source of one"), ([(0, 1, 2)], "page ids are wanted"),
+                        ([(0, 1.5)], "page ids are wanted"), ([(0, 1 << 40)], "page ids are wanted")):
         with pytest.raises(KernelError, match=text):
             K.copy_pages(pool, pairs)
     empty = K.attention_kv4(z(0, 256), cache, SimpleNamespace(block_table=z(1, 4, t=torch.int32), token_request=z(0, t=torch.int32),

@@ -118,6 +118,13 @@ def test_c_entry_points_refuse_before_they_touch_the_device():
     pairs = (ctypes.c_int * 4)(0, 1, 2, 8)
     rc, text = call("llm_copy_pages", at, 2, 8, 1024, pairs, 2, None)
     assert rc == -1 and "page 8" in text
+    for bad, text in (((0, 1, 2, 1), "page 1 is the destination of two copies"), ((0, 1, 1, 2), "page 1 is the source of one copy"),
+                      ((3, 3, 0, 1), "page 3 is the source of one copy"), ((5, 6, 6, 6), "page 6 is the")):
+        rc, said = call("llm_copy_pages", at, 2, 8, 1024, (ctypes.c_int * 4)(*bad), 2, None)
+        assert rc == -1 and text in said
+    many = [x for i in range(400) for x in (i, 1000 + i)] + [1399, 999]          # the last pair reads what the one before writes
+    rc, said = call("llm_copy_pages", at, 2, 2000, 1024, (ctypes.c_int * len(many))(*many), 401, None)
+    assert rc == -1 and "page 1399 is the source of one copy" in said
     # nothing to do is no error
     assert call("llm_copy_pages", at, 2, 8, 1024, pairs, 0, None)[0] == 0
 
