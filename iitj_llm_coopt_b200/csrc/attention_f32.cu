@@ -13,7 +13,7 @@
 //                         the keys, a number a thread, from value tiles that cp.async keeps ahead.  Bound by the chain's latency.
 // Measured in whole steps of the 1B shape (32 heads on 8 of 64 numbers, 16 layers), against one warp per token and head: a prompt of 777
 // tokens 33.7 -> 15.5 ms a step (attention 1290 -> about 150 us a layer), five requests of 300 to 900 tokens decoding 7.1 -> 2.3 ms.
-#include "common.cuh"
+#include "kv4.cuh"
 
 namespace {
 
@@ -28,6 +28,9 @@ __device__ __forceinline__ bool finite4(float4 v) {
     return big <= 3.402823466e38f && v.x == v.x && v.y == v.y && v.z == v.z && v.w == v.w;
 }
 
+template <bool PACKED> struct CacheOf { typedef float type; };
+template <> struct CacheOf<true> { typedef uint8_t type; };
+
 // The butterfly of warp_sum over 32 terms of which a thread holds c, c + 8, c + 16, c + 24 (c = its place among eight lanes).
 __device__ __forceinline__ float sum32(const float (&p)[4]) {
     float v = (p[0] + p[2]) + (p[1] + p[3]);
@@ -36,9 +39,32 @@ __device__ __forceinline__ float sum32(const float (&p)[4]) {
     return v;
 }
 
-template <int D>
+// The words of a quarter of a key and of its value in a packed cache (kv4.cuh): numbers 8 j .. 8 j + 7 of every group.
+template <int G> struct PackedQuarter { uint32_t k[G], kp[G], v[G], vp[G]; };
+
+template <int G> __device__ __forceinline__ void load_words(uint32_t (&w)[G], const uint8_t* at) {
+    if constexpr (G == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(at);
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(at);
+        w[0] = x.x; w[1] = x.y;
+    }
+}
+__device__ __forceinline__ void store_numbers(float* to, uint32_t word, uint32_t par) {
+    const float s = kv4_step(par), z = kv4_zero(par);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(s, __uint_as_float((word >> kv4_bit(e) & 15u) | 0x4b000000u) - 8388608.f, z);       // (2^23 + n - 2^23)
+    *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+
+// PACKED: the keys and values are a packed cache's numbers; four threads a key fetch its codes a tile ahead and write the numbers where
+// the other form's copies land.
+template <int D, bool PACKED>
 __global__ void __launch_bounds__(128)
-attn_f32_tile_kernel(const float* __restrict__ q, int q_stride, const float* __restrict__ cache, const int* __restrict__ block_table,
+attn_f32_tile_kernel(const float* __restrict__ q, int q_stride, const typename CacheOf<PACKED>::type* __restrict__ cache, const int* __restrict__ block_table,
                      int table_width, const int* __restrict__ tiles, int n_tiles, float* __restrict__ out, int out_stride, int heads,
                      int kv_heads, int page_size, int window, float scale) {
     pdl_trigger();
@@ -64,6 +90,32 @@ attn_f32_tile_kernel(const float* __restrict__ q, int q_stride, const float* __r
         if (r < rows) v = *reinterpret_cast<const float4*>(q + (size_t)(row0 + r) * q_stride + (size_t)h * D + c);
         *reinterpret_cast<float4*>(Qs + r * LDK + c) = v;
     }
+    constexpr int G = D / 32;
+    const size_t block_bytes = PACKED ? kv4_block_bytes(page_size, G) : 0;
+    PackedQuarter<G> quarter;
+    auto fetch_packed = [&](int k0) {
+        const int key = k0 + (tid >> 2), j = tid & 3;
+        if (key >= first && key <= last) {
+            const int lp = key / page_size, at = key - lp * page_size;
+            const uint8_t* block = reinterpret_cast<const uint8_t*>(cache) + ((size_t)table[lp] * kv_heads + hk) * block_bytes;
+            load_words<G>(quarter.k, block + at * 16 * G + 4 * G * j);
+            load_words<G>(quarter.kp, block + kv4_key_par(page_size, G) + at * 4 * G);
+            load_words<G>(quarter.v, block + kv4_value_codes(page_size, G) + at * 16 * G + 4 * G * j);
+            load_words<G>(quarter.vp, block + kv4_value_par(page_size, G) + at * 4 * G);
+        } else {
+#pragma unroll
+            for (int g = 0; g < G; ++g) quarter.k[g] = quarter.kp[g] = quarter.v[g] = quarter.vp[g] = 0u;
+        }
+    };
+    auto land_packed = [&](int buf) {
+        const int row = tid >> 2, j = tid & 3;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const uint32_t v = __byte_perm(quarter.v[g / 2], quarter.v[G / 2 + g / 2], (g & 1) ? 0x7632 : 0x5410);       // two half-words of a value row
+            store_numbers(Ks + ((size_t)buf * kTileK + row) * LDK + 32 * g + 8 * j, quarter.k[g], quarter.kp[g]);
+            store_numbers(Vs + ((size_t)buf * kTileK + row) * D + 32 * g + 8 * j, v, quarter.vp[g]);
+        }
+    };
     auto fetch = [&](int k0, int buf) {                // four threads a key: its row of the key plane and of the value plane
         const int j = tid >> 2, key = k0 + j;
         const bool live = key >= first && key <= last;
@@ -87,21 +139,28 @@ attn_f32_tile_kernel(const float* __restrict__ q, int q_stride, const float* __r
             for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
     }
     const int k_begin = first & ~(kTileK - 1);
-    fetch(k_begin, 0);
+    if constexpr (PACKED) fetch_packed(k_begin);
+    else fetch(k_begin, 0);
     int buf = 0;
     for (int k0 = k_begin; k0 <= last; k0 += kTileK, buf ^= 1) {
-        if (k0 + kTileK <= last) {
-            fetch(k0 + kTileK, buf ^ 1);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-        } else {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-        }
-        // values that are not finite must not reach a query that does not see them (0 * inf): looked for by the thread that fetched them
         bool odd = false;
+        if constexpr (PACKED) {
+            land_packed(buf);
+            if (k0 + kTileK <= last) fetch_packed(k0 + kTileK);
+            __syncthreads();                               // (a packed cache's values are finite)
+        } else {
+            if (k0 + kTileK <= last) {
+                fetch(k0 + kTileK, buf ^ 1);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+            // values that are not finite must not reach a query that does not see them (0 * inf): looked for by the thread that fetched them
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-            odd |= !finite4(*reinterpret_cast<const float4*>(Vs + ((size_t)buf * kTileK + (tid >> 2)) * D + ((tid & 3) + 4 * i) * 4));
-        odd = __syncthreads_or(odd);
+            for (int i = 0; i < D / 16; ++i)
+                odd |= !finite4(*reinterpret_cast<const float4*>(Vs + ((size_t)buf * kTileK + (tid >> 2)) * D + ((tid & 3) + 4 * i) * 4));
+            odd = __syncthreads_or(odd);
+        }
 
         // scores: queries rg + 16 i, keys cg + 8 j
         const float* Kb = Ks + (size_t)buf * kTileK * LDK;
@@ -354,7 +413,26 @@ LLM_API int llm_attention_f32_tiles(const float* q, int q_stride, const float* c
         LLM_CHECK_LAUNCH("attention_f32_tiles");
         return 0;
     };
-    return head_dim == 64 ? go(attn_f32_tile_kernel<64>, tile_smem<64>()) : go(attn_f32_tile_kernel<128>, tile_smem<128>());
+    return head_dim == 64 ? go(attn_f32_tile_kernel<64, false>, tile_smem<64>()) : go(attn_f32_tile_kernel<128, false>, tile_smem<128>());
+}
+
+// The same over a packed cache layer (kv4.cuh).
+LLM_API int llm_attention_kv4_f32_tiles(const float* q, int q_stride, const void* cache, const int* block_table, int table_width,
+                                        const int* tiles, int n_tiles, float* out, int out_stride, int heads, int kv_heads, int head_dim,
+                                        int page_size, int window, float scale, cudaStream_t stream) {
+    if (n_tiles == 0) return 0;
+    if (int rc = check(heads, kv_heads, head_dim, "attention_kv4_f32_tiles")) return rc;
+    if (!kv4_geometry(head_dim, page_size)) LLM_FAIL(-1, "attention_kv4_f32_tiles: page_size %d is not a multiple of 4", page_size);
+    if (n_tiles > 65535) LLM_FAIL(-1, "attention_kv4_f32_tiles: %d tiles are too many for one launch", n_tiles);
+    const dim3 grid(heads, n_tiles);
+    auto go = [&](auto kern, size_t smem) {
+        if (int rc = set_smem(kern, smem, "attention_kv4_f32_tiles")) return rc;
+        llm_launch(kern, grid, 128, smem, stream, q, q_stride, (const uint8_t*)cache, block_table, table_width, tiles, n_tiles, out, out_stride,
+                   heads, kv_heads, page_size, window, scale);
+        LLM_CHECK_LAUNCH("attention_kv4_f32_tiles");
+        return 0;
+    };
+    return head_dim == 64 ? go(attn_f32_tile_kernel<64, true>, tile_smem<64>()) : go(attn_f32_tile_kernel<128, true>, tile_smem<128>());
 }
 
 // items: the token rows of single decoded tokens.

@@ -1,38 +1,39 @@
 // Attention over the packed key/value cache (format: kv4.cuh): the general kernel.
 //
 // Any head size (a multiple of 32 up to 256), any page size (a multiple of 4), both engine types, any mix of prompt portions and
-// single tokens: one block a token row and key/value head, for up to eight of the group's query heads at a time.  Every number of the
+// single tokens: one block a token row and key/value head, for up to four of the group's query heads at a time.  Every number of the
 // cache is taken apart once per block, as z + s n in float32, and enters float32 products.
 //
 //   scores   a lane is a key: it reads its key's words and adds q . k for the block's query heads, q broadcast from shared memory
-//   softmax  running maximum and sum a head and warp (warp w takes the 32-key chunks w, w + 4, ..., so the four warps see different keys)
+//   softmax  running maximum and sum a head and warp (a block's warps take the 32-key chunks in turn, so they see different keys)
 //   values   a lane is four numbers of the value head (a half-word of codes), the chunk's probabilities broadcast from shared memory
-// and at the end the four warps' sums are joined.  Keys outside [lo, pos] are not read.
+// and at the end the warps' sums are joined.  Keys outside [lo, pos] are not read.
 #include "kv4.cuh"
 
 namespace {
 
-constexpr int kGenThreads = 128, kGenWarps = 4, kGenHeads = 8;
+constexpr int kGenHeads = 4;
 
 template <typename T> __device__ __forceinline__ T of_float(float v) { return from_f32<T>(v); }
 
-template <typename T>
-__global__ void __launch_bounds__(kGenThreads)
+// GT: groups of a head as a constant (a key's words then come in a few wide loads, all asked for at once), or 0.
+template <typename T, int WARPS, int GT>
+__global__ void __launch_bounds__(32 * WARPS)
 attn_kv4_general_kernel(const T* __restrict__ q, int q_stride, const uint8_t* __restrict__ cache, const int* __restrict__ block_table,
-                        int table_width, const int* __restrict__ token_request, const int* __restrict__ positions, T* __restrict__ out,
+                        int table_width, const int* __restrict__ rows, const int* __restrict__ token_request, const int* __restrict__ positions, T* __restrict__ out,
                         int out_stride, int heads, int kv_heads, int head_dim, int page_size, int window, float sl) {
     pdl_trigger();
     pdl_wait();
     __shared__ __align__(16) float sq[kGenHeads][kKv4MaxDim];
-    __shared__ float sp[kGenWarps][kGenHeads][32];
-    __shared__ float sm[kGenWarps][kGenHeads], sl_sum[kGenWarps][kGenHeads];
-    const int t = blockIdx.x, hk = blockIdx.y, D = head_dim, G = D / 32, group = heads / kv_heads;
+    __shared__ float sp[WARPS][kGenHeads][32];
+    __shared__ float sm[WARPS][kGenHeads], sl_sum[WARPS][kGenHeads];
+    const int t = rows ? rows[blockIdx.x] : blockIdx.x, hk = blockIdx.y, D = GT ? 32 * GT : head_dim, G = GT ? GT : D / 32, group = heads / kv_heads;
     const int h0 = hk * group + blockIdx.z * kGenHeads, nh = min(kGenHeads, group - (int)blockIdx.z * kGenHeads);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int pos = positions[t], lo = window > 0 ? max(0, pos - window + 1) : 0;
     const int* table = block_table + (size_t)token_request[t] * table_width;
     const size_t block_bytes = kv4_block_bytes(page_size, G);
-    for (int i = threadIdx.x; i < kGenHeads * D; i += kGenThreads) {
+    for (int i = threadIdx.x; i < kGenHeads * D; i += (32 * WARPS)) {
         const int h = i / D, c = i - h * D;
         sq[h][c] = h < nh ? to_f32(q[(size_t)t * q_stride + (size_t)(h0 + h) * D + c]) * sl : 0.f;       // (scores in log2 units)
     }
@@ -46,30 +47,40 @@ attn_kv4_general_kernel(const T* __restrict__ q, int q_stride, const uint8_t* __
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[0][h][e] = o[1][h][e] = 0.f;
     }
-    for (int k0 = lo + warp * 32; k0 <= pos; k0 += kGenWarps * 32) {
+    for (int k0 = lo + warp * 32; k0 <= pos; k0 += WARPS * 32) {
         const int n = min(32, pos + 1 - k0), key = k0 + min(lane, n - 1);
-        const int lp = key / page_size, off = key - lp * page_size;
-        const uint8_t* block = cache + ((size_t)table[lp] * kv_heads + hk) * block_bytes;
+        const int lp = key / page_size, off = key - lp * page_size, page = table[lp];
+        const uint8_t* block = cache + ((size_t)page * kv_heads + hk) * block_bytes;
         const uint32_t* codes = reinterpret_cast<const uint32_t*>(block + (size_t)off * 16 * G);
         const uint32_t* par = reinterpret_cast<const uint32_t*>(block + kv4_key_par(page_size, G) + (size_t)off * 4 * G);
         float s[kGenHeads];
 #pragma unroll
         for (int h = 0; h < kGenHeads; ++h) s[h] = 0.f;
-        for (int g = 0; g < G; ++g) {
-            const uint32_t p = par[g];
+        auto add_word = [&](uint32_t w, uint32_t p, int g, int j) {
             const float step = kv4_step(p), zero = kv4_zero(p);
+            float x[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t w = codes[j * G + g];
-                float x[8];
+            for (int e = 0; e < 8; ++e) x[e] = fmaf(step, (float)((w >> kv4_bit(e)) & 15u), zero);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = fmaf(step, (float)((w >> kv4_bit(e)) & 15u), zero);
-#pragma unroll
-                for (int h = 0; h < kGenHeads; ++h) {
-                    const float4 a = *reinterpret_cast<const float4*>(&sq[h][32 * g + 8 * j]), b = *reinterpret_cast<const float4*>(&sq[h][32 * g + 8 * j + 4]);
-                    s[h] += ((a.x * x[0] + a.y * x[1]) + (a.z * x[2] + a.w * x[3])) + ((b.x * x[4] + b.y * x[5]) + (b.z * x[6] + b.w * x[7]));
-                }
+            for (int h = 0; h < kGenHeads; ++h) {
+                const float4 a = *reinterpret_cast<const float4*>(&sq[h][32 * g + 8 * j]), b = *reinterpret_cast<const float4*>(&sq[h][32 * g + 8 * j + 4]);
+                s[h] += ((a.x * x[0] + a.y * x[1]) + (a.z * x[2] + a.w * x[3])) + ((b.x * x[4] + b.y * x[5]) + (b.z * x[6] + b.w * x[7]));
             }
+        };
+        if constexpr (GT > 0) {
+            struct alignas(4 * GT) Words { uint32_t w[GT]; };
+            const Words p = *reinterpret_cast<const Words*>(par);
+            Words c[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c[j] = reinterpret_cast<const Words*>(codes)[j];
+#pragma unroll
+            for (int g = 0; g < GT; ++g)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) add_word(c[j].w[g], p.w[g], g, j);
+        } else {
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) add_word(codes[j * G + g], par[g], g, j);
         }
         __syncwarp();                                    // the chunk before is done with sp
 #pragma unroll
@@ -85,9 +96,10 @@ attn_kv4_general_kernel(const T* __restrict__ q, int q_stride, const uint8_t* __
             sp[warp][h][lane] = p;
         }
         __syncwarp();
+#pragma unroll 4
         for (int i = 0; i < n; ++i) {
-            const int kk = k0 + i, vp = kk / page_size, voff = kk - vp * page_size;
-            const uint8_t* vb = cache + ((size_t)table[vp] * kv_heads + hk) * block_bytes;
+            const int voff = __shfl_sync(0xffffffffu, off, i);
+            const uint8_t* vb = cache + ((size_t)__shfl_sync(0xffffffffu, page, i) * kv_heads + hk) * block_bytes;
             const uint16_t* vc = reinterpret_cast<const uint16_t*>(vb + kv4_value_codes(page_size, G) + (size_t)voff * 16 * G);
             const uint32_t* vpar = reinterpret_cast<const uint32_t*>(vb + kv4_value_par(page_size, G) + (size_t)voff * 4 * G);
 #pragma unroll
@@ -106,6 +118,11 @@ attn_kv4_general_kernel(const T* __restrict__ q, int q_stride, const uint8_t* __
             }
         }
     }
+    auto top_of = [&](int h) {
+        float top = sm[0][h];
+        for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm[w][h]);
+        return top;
+    };
 #pragma unroll
     for (int h = 0; h < kGenHeads; ++h) {
         l[h] = warp_sum(l[h]);
@@ -113,10 +130,10 @@ attn_kv4_general_kernel(const T* __restrict__ q, int q_stride, const uint8_t* __
     }
     __syncthreads();
     // joined over the warps, one after another, into the query rows' place
-    for (int w = 0; w < kGenWarps; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
         if (warp == w) {
             for (int h = 0; h < nh; ++h) {
-                const float top = fmaxf(fmaxf(sm[0][h], sm[1][h]), fmaxf(sm[2][h], sm[3][h]));
+                const float top = top_of(h);
                 const float f = sm[w][h] == -INFINITY ? (sl_sum[w][h] == 0.f ? 0.f : 1.f) : exp2f(sm[w][h] - top);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -137,31 +154,39 @@ attn_kv4_general_kernel(const T* __restrict__ q, int q_stride, const uint8_t* __
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < nh * D; i += kGenThreads) {
+    for (int i = threadIdx.x; i < nh * D; i += (32 * WARPS)) {
         const int h = i / D, c = i - h * D;
-        const float top = fmaxf(fmaxf(sm[0][h], sm[1][h]), fmaxf(sm[2][h], sm[3][h]));
+        const float top = top_of(h);
         float sum = 0.f;
-        for (int w = 0; w < kGenWarps; ++w) sum += sl_sum[w][h] * (sm[w][h] == -INFINITY ? (sl_sum[w][h] == 0.f ? 0.f : 1.f) : exp2f(sm[w][h] - top));
+        for (int w = 0; w < WARPS; ++w) sum += sl_sum[w][h] * (sm[w][h] == -INFINITY ? (sl_sum[w][h] == 0.f ? 0.f : 1.f) : exp2f(sm[w][h] - top));
         out[(size_t)t * out_stride + (size_t)(h0 + h) * D + c] = of_float<T>(sq[h][c] / sum);
     }
 }
 
 }  // namespace
 
-// q: [tokens, q_stride], head h at columns [h * head_dim, ...); cache: pages of kv_heads blocks (kv4.cuh).
+// rows: [n_rows] the token rows to work on, null: rows 0 .. n_rows - 1.  q: [tokens, q_stride], head h at columns [h * head_dim, ...); cache: pages of kv_heads blocks (kv4.cuh).
 LLM_API int llm_attention_kv4_general(const void* q, int q_stride, const void* cache, const int* block_table, int table_width,
-                                      const int* token_request, const int* positions, void* out, int out_stride, int dtype, int tokens, int heads,
+                                      const int* rows, int n_rows, const int* token_request, const int* positions, void* out, int out_stride, int dtype, int heads,
                                       int kv_heads, int head_dim, int page_size, int window, float scale, cudaStream_t stream) {
-    if (tokens == 0) return 0;
+    if (n_rows == 0) return 0;
     if (!kv4_geometry(head_dim, page_size) || kv_heads <= 0 || heads % kv_heads)
         LLM_FAIL(-1, "attention_kv4: heads %d / kv_heads %d / head_dim %d / page %d not supported", heads, kv_heads, head_dim, page_size);
     const int tiles = (heads / kv_heads + kGenHeads - 1) / kGenHeads;
     if (kv_heads > 65535 || tiles > 65535) LLM_FAIL(-1, "attention_kv4: too many heads");
     return llm_dispatch_dtype(dtype, [&](auto tag) {
         using T = decltype(tag);
-        llm_launch(attn_kv4_general_kernel<T>, dim3(tokens, kv_heads, tiles), kGenThreads, 0, stream, (const T*)q, q_stride, (const uint8_t*)cache,
-                   block_table, table_width, token_request, positions, (T*)out, out_stride, heads, kv_heads, head_dim, page_size, window,
-                   scale * 1.4426950408889634f);
+        auto go = [&](auto kernel, int warps) {
+            llm_launch(kernel, dim3(n_rows, kv_heads, tiles), 32 * warps, 0, stream, (const T*)q, q_stride, (const uint8_t*)cache, block_table,
+                       table_width, rows, token_request, positions, (T*)out, out_stride, heads, kv_heads, head_dim, page_size, window,
+                       scale * 1.4426950408889634f);
+        };
+        // Few blocks: more warps share a block's keys.  Five requests of 300 to 900 keys, 32 / 8 heads of 64 numbers in float32, were 99 us
+        // with four warps a block and are 41 with sixteen, wide loads of a key's words and values asked for four at a time.
+        const bool few = (long long)n_rows * kv_heads * tiles <= 512;
+        if (head_dim == 64) { if (few) go(attn_kv4_general_kernel<T, 16, 2>, 16); else go(attn_kv4_general_kernel<T, 4, 2>, 4); }
+        else if (head_dim == 128) { if (few) go(attn_kv4_general_kernel<T, 16, 4>, 16); else go(attn_kv4_general_kernel<T, 4, 4>, 4); }
+        else { if (few) go(attn_kv4_general_kernel<T, 16, 0>, 16); else go(attn_kv4_general_kernel<T, 4, 0>, 4); }
         LLM_CHECK_LAUNCH("attention_kv4");
         return 0;
     });

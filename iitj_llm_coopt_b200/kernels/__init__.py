@@ -49,8 +49,8 @@ _SIGNATURES = {
     "llm_rope_store_kv4": [_c_void_p, _c_void_p, _c_int, ctypes.c_longlong, _c_void_p, ctypes.c_longlong, _c_void_p, _c_void_p, _c_void_p,
                            _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p],
     "llm_kv4_read": [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p],
-    "llm_attention_kv4_general": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
-                                  _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p],
+    "llm_attention_kv4_general": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
+                                  _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p],
     "llm_attention_kv4_single_supported": [_c_int, _c_int, _c_int, _c_int],
     "llm_attention_kv4_single_tile": [],
     "llm_attention_kv4_single_warps": [],
@@ -60,6 +60,8 @@ _SIGNATURES = {
     "llm_attention_kv4_prompt_supported": [_c_int, _c_int, _c_int, _c_int],
     "llm_attention_kv4_prompt": [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int,
                                  _c_int, _c_int, _c_int, _c_float, _c_int, _c_void_p, _c_void_p, _c_void_p],
+    "llm_attention_kv4_f32_tiles": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_int,
+                                    _c_int, _c_int, _c_float, _c_void_p],
     "llm_copy_pages": [_c_void_p, _c_int, ctypes.c_longlong, ctypes.c_longlong, _c_void_p, _c_int, _c_void_p],
     "llm_silu_mul": [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p],
     "llm_scale_f32": [_c_void_p, _c_float, ctypes.c_longlong, _c_void_p],
@@ -908,22 +910,31 @@ class Kernels:
             scale = 1.0 / math.sqrt(head_dim)
         if not tokens:
             return out
-        plan = None
-        if q.dtype == torch.bfloat16 and getattr(meta, "query_lens", None) is not None and q.data_ptr() % 16 == 0 and q.shape[1] % 8 == 0:
+        # the fast forms: of the prompt portions (bfloat16 on tcgen05, float32 by query tiles), of the single tokens (bfloat16)
+        plan, portions, singles = None, False, False
+        if getattr(meta, "query_lens", None) is not None and q.data_ptr() % 16 == 0 and q.shape[1] % 8 == 0 and out.data_ptr() % 16 == 0:
             plan = attention_plan(meta, q.device)
-        shape = (heads, kv_heads, head_dim, page_size)
-        forms = self._kv4_forms.get(shape)
-        if forms is None:
-            forms = self._kv4_forms[shape] = (self.lib.llm_attention_kv4_prompt_supported(*shape), self.lib.llm_attention_kv4_single_supported(*shape))
-        if plan is not None and (not plan.n_tiles or forms[0]) and (not plan.n_items or forms[1]):
-            if plan.n_tiles:
+            shape = (heads, kv_heads, head_dim, page_size)
+            forms = self._kv4_forms.get(shape)
+            if forms is None:
+                forms = self._kv4_forms[shape] = (self.lib.llm_attention_kv4_prompt_supported(*shape), self.lib.llm_attention_kv4_single_supported(*shape))
+            portions, singles = forms[0] and plan.n_tiles <= 65535, forms[1] and q.dtype == torch.bfloat16 and plan.n_items <= 65535
+        rows, n_rows = None, tokens           # what is left to the general kernel
+        if plan is not None and (portions or not plan.n_tiles):
+            if plan.n_tiles and q.dtype == torch.bfloat16:
                 self._kv4_prompt(q, cache_layer, meta, plan, out, *shape, int(window), float(scale))
-            if plan.n_items:
+            elif plan.n_tiles:
+                self._call("llm_attention_kv4_f32_tiles", _ptr(q), q.shape[1], _ptr(cache_layer), _ptr(meta.block_table), meta.block_table.shape[1],
+                           _ptr(plan.tiles), plan.n_tiles, _ptr(out), out.shape[1], heads, kv_heads, head_dim, page_size, int(window),
+                           float(scale), self._stream())
+            rows, n_rows = plan.items, plan.n_items
+            if n_rows and singles:
                 self._kv4_single(q, cache_layer, meta, plan, out, *shape, int(window), float(scale))
-        else:
+                n_rows = 0
+        if n_rows:
             self._call("llm_attention_kv4_general", _ptr(q), q.shape[1], _ptr(cache_layer), _ptr(meta.block_table), meta.block_table.shape[1],
-                       _ptr(meta.token_request), _ptr(meta.positions), _ptr(out), out.shape[1], DTYPE_CODE[q.dtype], tokens, heads, kv_heads,
-                       head_dim, page_size, int(window), float(scale), self._stream())
+                       _ptr(rows), n_rows, _ptr(meta.token_request), _ptr(meta.positions), _ptr(out), out.shape[1], DTYPE_CODE[q.dtype],
+                       heads, kv_heads, head_dim, page_size, int(window), float(scale), self._stream())
         return out
 
     def _kv4_prompt(self, q, cache_layer, meta, plan, out, heads, kv_heads, head_dim, page_size, window, scale):
