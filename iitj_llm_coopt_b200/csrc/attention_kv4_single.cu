@@ -16,9 +16,11 @@
 //            over those gives the score's part as s S + z sum q - s sum (1024 or 64) q.  The last two terms of all groups are two more
 //            products: one operand are the stored (s, z) words as they lie, the other one the sums of q (as three bfloat16 each).  Nothing
 //            of the key is rounded.
-//   values   the transposed product, 16 numbers x 8 heads over 16 keys: the operand is n itself (128 + n - 128, exact), the other one
-//            p s, p rounded to bfloat16 and the product rounded again, a group at a time.  The zero points' part sum p z and the sum of p
-//            are one more product, of rows z_g and 1, with the same p.
+//   values   the transposed product, 16 numbers x 8 heads over 16 keys: the operand is n - 8 (128 + n - 136, exact), the other one
+//            p s, p rounded to bfloat16 and the product rounded again, a group at a time.  The middles z + 8 s (rounded to bfloat16: they
+//            are small beside the numbers) and the sum of p are one more product, of rows of middles and of ones, with the same p.
+//            (About the zero points, with n for n - 8, the two parts nearly cancel over a long context: at 32000 keys the result was 5.2e-3
+//            off the one in 64 bits, with 8 s and z summed apart 2.6e-3; it is AFTER, of which bfloat16's last rounding alone makes 1.7e-3.)
 // The order of codes in a row (kv4.cuh) is the order in which these instructions' lanes want them: no shuffle, one 4 G-byte load of a
 // key row and one 2 G-byte load of a value row per lane.
 #include "kv4.cuh"
@@ -91,11 +93,18 @@ template <uint32_t MASK> __device__ __forceinline__ uint32_t and_or(uint32_t w, 
 // Two codes (bits 0-3 and 16-19 of w) as the float16 numbers 1024 + n; two codes of bits 4-7 and 20-23 as 64 + n.
 __device__ __forceinline__ uint32_t half_codes_low(uint32_t w) { return and_or<0x000f000fu>(w, 0x64006400u); }
 __device__ __forceinline__ uint32_t half_codes_high(uint32_t w) { return and_or<0x00f000f0u>(w, 0x54005400u); }
-// Two codes (bits 0-3 and 16-19 of w) as the bfloat16 numbers n: 128 + n - 128.
+// Two codes (bits 0-3 and 16-19 of w) as the bfloat16 numbers n - 8: 128 + n - 136.
 __device__ __forceinline__ uint32_t codes(uint32_t w) {
     const uint32_t x = and_or<0x000f000fu>(w, 0x43004300u);
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(128.f));
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(136.f));
     return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+// z + 8 s of two tokens' (s, z) words.
+__device__ __forceinline__ uint32_t middles(uint32_t a, uint32_t b) {
+    const uint32_t s = __byte_perm(a, b, 0x5410), z = __byte_perm(a, b, 0x7632);
+    const __nv_bfloat162 m = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&s), __float2bfloat162_rn(8.f), *reinterpret_cast<const __nv_bfloat162*>(&z));
+    return *reinterpret_cast<const uint32_t*>(&m);
 }
 
 template <int G> struct alignas(4 * G) Words { uint32_t w[G]; };
@@ -338,10 +347,10 @@ attn_kv4_single_kernel(const SingleArgs a) {
             const uint32_t p0 = transposed8x8(pack_pair(ex2(t[u][0]), ex2(t[u][1]))), p1 = transposed8x8(pack_pair(ex2(t[u][2]), ex2(t[u][3])));
             const unsigned char* vu = base + 16 * u * 16 * G;
             const unsigned char* pu = base + 16 * u * 4 * G;
-            {   // zero points' part and the sum: rows z_g and 1 over the 16 tokens, times p
-                const uint32_t ab = __byte_perm(lds<uint32_t>(pu + vz_at), lds<uint32_t>(pu + vz_at + 4 * 4 * G), 0x7632);
-                const uint32_t cd = __byte_perm(lds<uint32_t>(pu + vz_at + 8 * 4 * G), lds<uint32_t>(pu + vz_at + 12 * 4 * G), 0x7632);
-                mma16816(oz, (ab & z_keep) | z_add, 0u, (cd & z_keep) | z_add, 0u, p0, p1);
+            {   // rows of the groups' middles, and a row of ones, over the 16 tokens, times p
+                const uint32_t wa = lds<uint32_t>(pu + vz_at), wb = lds<uint32_t>(pu + vz_at + 4 * 4 * G);
+                const uint32_t wc = lds<uint32_t>(pu + vz_at + 8 * 4 * G), wd = lds<uint32_t>(pu + vz_at + 12 * 4 * G);
+                mma16816(oz, (middles(wa, wb) & z_keep) | z_add, 0u, (middles(wc, wd) & z_keep) | z_add, 0u, p0, p1);
             }
             const unsigned char* wu = pu + kValuePar + j * 4 * G;
             const Words<G> wa = lds<Words<G>>(wu), wb = lds<Words<G>>(wu + 4 * 4 * G), wc = lds<Words<G>>(wu + 8 * 4 * G), wd = lds<Words<G>>(wu + 12 * 4 * G);
@@ -382,7 +391,7 @@ attn_kv4_single_kernel(const SingleArgs a) {
     }
 
     // ---- the warps' sums joined, then the blocks' --------------------------------------------------------------------------
-    // row g of oz is the zero points' part of group g, row G the sum: this lane's columns are heads 2 j and 2 j + 1
+    // row g of oz is the middles' part of group g, row G the sum of p: this lane's columns are heads 2 j and 2 j + 1
     float zg[G][2], l[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
