@@ -24,13 +24,25 @@
 // statistics as the mma.sync kernel of attention_bf16.cu, which remains for page sizes that do not divide 128.
 //
 // The same kernel over a packed cache (kv4.cuh; any page size that is a multiple of 4): four more warps take the codes apart and write the
-// tiles that TMA would have brought, the cache's numbers z + s n rounded to bfloat16 (one multiply-and-add).  Both heads of a CTA use
-// them, and the work hides beside the softmax, which leaves two thirds of the issue slots free.
+// tiles that TMA would have brought, the cache's numbers z + s n rounded once (one multiply-and-add).  Both heads of a CTA use them, and
+// most of the work hides beside the softmax, which leaves two thirds of the issue slots free.  A bfloat16 would be a second rounding of
+// numbers that are coarse already, 2^-9 of keys whose few loud numbers weigh most (5.1e-3 off the result in 64 bits at 8000 keys); so the
+// products' operands are float16 there, within its range by powers of two:
+//   queries  every row over its largest number's (the softmax's warps convert the tile as it lands, a row a thread; its scale takes the
+//            power back): exact
+//   keys     over the power of two that holds a tile's largest |z| and 15 s (warp 0 reads the tiles' parameters ahead and leaves both
+//            exponents of a tile in a ring of words, `tops`); the scale of the tile's scores takes the power back
+//   values   over such a power 2^e as well.  P of the tile is taken times 2^e, so O needs nothing; l takes it back.  The reference
+//            M follows the scores plus e: what float16 flushes lies 2^-29 below the tile's largest value, or 2^-32 below the row's
+//            largest product
+// P must not pass float16's range before its row's reference moves, so every tile takes the two passes over its scores.
 //
 // Every mbarrier wait is bounded; a wait that runs out records a code (llm_attention_tcgen05_status)
 // and the CTA falls through to its teardown, where the tensor memory is freed.
 #include "kv4.cuh"
 #include "tcgen05_common.cuh"
+
+#include <cuda_fp16.h>
 
 #include <cstdlib>
 #include <type_traits>
@@ -62,6 +74,15 @@ __device__ __forceinline__ void attn_give_up(int code) { atomicCAS(&g_attn_statu
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
+}
+
+template <bool HALF> __device__ __forceinline__ uint32_t pack_operand(float lo, float hi) {
+    if constexpr (HALF) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        return pack2(lo, hi);
+    }
 }
 
 __device__ __forceinline__ float ex2(float x) {          // 2^x; one MUFU instruction
@@ -143,9 +164,9 @@ __device__ __forceinline__ float chunk_max(const uint32_t (&r)[32], int k0, int 
     return fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
 }
 
-// P = 2^(S * sl - mu) of 32 scores, packed as 16 columns of two bfloat16; adds to four partial sums (sum[i] takes the
+// P = 2^(S * sl - mu) of 32 scores, packed as 16 columns of two bfloat16 (HALF: float16); adds to four partial sums (sum[i] takes the
 // keys i, i + 4, ... of the chunk in both forms, so a row's sum does not depend on whether its tile was masked).
-template <bool MASK>
+template <bool MASK, bool HALF>
 __device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], uint32_t (&packed)[16], float sl, float mu, int k0, int row_pos,
                                           int row_lo, float (&sum)[4]) {
     if constexpr (!MASK) {
@@ -159,8 +180,8 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], uint32_t (&pa
             const float p0 = ex2(x0), p1 = ex2(x1), p2 = ex2(x2), p3 = ex2(x3);
             s01 = add_pair(s01, pair_of(p0, p1));
             s23 = add_pair(s23, pair_of(p2, p3));
-            packed[c >> 1] = pack2(p0, p1);
-            packed[(c >> 1) + 1] = pack2(p2, p3);
+            packed[c >> 1] = pack_operand<HALF>(p0, p1);
+            packed[(c >> 1) + 1] = pack_operand<HALF>(p2, p3);
         }
         split_pair(s01, sum[0], sum[1]);
         split_pair(s23, sum[2], sum[3]);
@@ -175,26 +196,48 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], uint32_t (&pa
             if (key + 2 > row_pos || key + 2 < row_lo) p2 = 0.f;
             if (key + 3 > row_pos || key + 3 < row_lo) p3 = 0.f;
             sum[0] += p0; sum[1] += p1; sum[2] += p2; sum[3] += p3;
-            packed[c >> 1] = pack2(p0, p1);
-            packed[(c >> 1) + 1] = pack2(p2, p3);
+            packed[c >> 1] = pack_operand<HALF>(p0, p1);
+            packed[(c >> 1) + 1] = pack_operand<HALF>(p2, p3);
         }
     }
 }
 
-// The eight numbers of a code word (kv4.cuh, key row), z + s n rounded to bfloat16.
-__device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t par) {
-    const uint32_t s2 = __byte_perm(par, par, 0x1010), z2 = __byte_perm(par, par, 0x3232);
+// The eight numbers of a code word (kv4.cuh, key row) times `down`, a power of two, z + s n rounded to float16.
+__device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t par, uint32_t down) {
+    const __nv_bfloat162 p = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&par), *reinterpret_cast<const __nv_bfloat162*>(&down));
+    const uint32_t pb = *reinterpret_cast<const uint32_t*>(&p);
+    const __half2 sz = __floats2half2_rn(kv4_step(pb), kv4_zero(pb)), s2 = __low2half2(sz), z2 = __high2half2(sz);
     uint32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+        // codes at bits 0 and 16 as 1024 + n, codes at bits 4 and 20 as 64 + n, exact
         uint32_t x;
-        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w >> (4 * i)), "n"(0x000f000f), "r"(0x43004300u));      // 128 + n, exact
-        const __nv_bfloat162 n = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(128.f));
-        const __nv_bfloat162 v = __hfma2(n, *reinterpret_cast<const __nv_bfloat162*>(&s2), *reinterpret_cast<const __nv_bfloat162*>(&z2));
+        if (i & 1) asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(i & 2 ? w >> 8 : w), "n"(0x00f000f0), "r"(0x54005400u));
+        else asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(i & 2 ? w >> 8 : w), "n"(0x000f000f), "r"(0x64006400u));
+        const __half2 n = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(i & 1 ? 64.f : 1024.f));
+        const __half2 v = __hfma2(n, s2, z2);
         r[i] = *reinterpret_cast<const uint32_t*>(&v);
     }
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
+
+constexpr int kTopRing = 8;               // words of tiles ahead
+constexpr float kPackedP = 7.f;           // P times 2^7 (in log2 units), at most 2^15 with a reference that lags by kRescaleStep
+
+// A tile's word: the biased exponents of its largest key and value, and its number (from 1, modulo 2^16), by which it is known.
+__device__ __forceinline__ bool top_wait(const volatile uint32_t* tops, int j, uint32_t& word) {
+    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+        word = tops[j % kTopRing];
+        if (word >> 16 == ((uint32_t)(j + 1) & 0xffffu)) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ uint32_t top_keys(uint32_t word) { return word & 0xffu; }
+__device__ __forceinline__ uint32_t top_values(uint32_t word) { return word >> 8 & 0xffu; }
+// 2^(14 - e) of an exponent, and its inverse
+__device__ __forceinline__ float top_down(uint32_t e8) { return __uint_as_float((268u - e8) << 23); }
+__device__ __forceinline__ float top_up(uint32_t e8) { return __uint_as_float((e8 - 14u) << 23); }
+constexpr uint32_t kKeyLeast = 60u, kValueLeast = 100u;      // numbers all below 2^-67 or 2^-27 are taken as if one were that large
 
 struct AttnArgs {
     const int* block_table;
@@ -226,7 +269,9 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     // Three stages for the values: a value tile is handed back only when both heads' P V of its keys are done, one
     // tile's time after the keys' stage, and with two stages its successor's boxes came in about 300 clocks late every tile.
     unsigned char* v_tile[3] = {base + 4 * kTileBytes, base + 5 * kTileBytes, base + 6 * kTileBytes};   // (the last only with three stages)
-    __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], v_full[kVStages], v_empty[kVStages], s_full[2], p_full[2], o_done[2];
+    __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], v_full[kVStages], v_empty[kVStages], s_full[2], p_full[2], o_done[2], q_ready[2];
+    __shared__ volatile uint32_t tops[kTopRing];
+    __shared__ volatile int tops_read[2 * kGroupThreads / 32];       // tiles whose words a softmax warp has taken
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int failed;
 
@@ -262,7 +307,9 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         for (int s = 0; s < 2; ++s) {
             mbar_init(&k_full[s], PACKED ? kUnpackWarps : 1); mbar_init(&k_empty[s], 1);
             mbar_init(&s_full[s], 1); mbar_init(&p_full[s], kGroupThreads / 32); mbar_init(&o_done[s], 1);
+            if (PACKED) mbar_init(&q_ready[s], kGroupThreads / 32);
         }
+        for (int s = 0; PACKED && s < kTopRing; ++s) { tops[s] = 0u; tops_read[s] = 0; }
         for (int s = 0; s < kVStages; ++s) { mbar_init(&v_full[s], PACKED ? kUnpackWarps : 1); mbar_init(&v_empty[s], 1); }
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -292,6 +339,53 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const int* table = a.block_table + (size_t)req * a.table_width;
         const int ps = a.page_size, pages_per_tile = kKeys / ps;
         int page = 0;
+        if constexpr (PACKED) {
+            // ---- the exponents of the tiles to come: lane x reads the parameters of keys 4 x .. 4 x + 3 of a tile -------------------------
+            constexpr int G = D / 32;
+            const size_t block_bytes = kv4_block_bytes(ps, G);
+            const uint8_t* cache = a.packed + (size_t)hk * block_bytes + ps * 16 * G;
+            const size_t page_bytes = (size_t)a.kv_heads * block_bytes;
+            struct Par { uint32_t k[4][G], v[4][G]; } par;
+            auto quad_of = [&](int j) { return min(max(k_begin + j * kKeys + 4 * lane, lo0 & ~3), pos_last & ~3); };
+            auto fetch = [&](int j, int page) {
+                const int quad = quad_of(j), off = quad - quad / ps * ps;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = off + min(max(quad + i, lo0), pos_last) - quad;       // (a row outside the reach may hold anything)
+                    const uint8_t* from = cache + (size_t)page * page_bytes + at * 4 * G;
+                    if constexpr (G == 4) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(from), y = *reinterpret_cast<const uint4*>(from + ps * 20 * G);
+                        par.k[i][0] = x.x; par.k[i][1] = x.y; par.k[i][2] = x.z; par.k[i][3] = x.w;
+                        par.v[i][0] = y.x; par.v[i][1] = y.y; par.v[i][2] = y.z; par.v[i][3] = y.w;
+                    } else {
+                        const uint2 x = *reinterpret_cast<const uint2*>(from), y = *reinterpret_cast<const uint2*>(from + ps * 20 * G);
+                        par.k[i][0] = x.x; par.k[i][1] = x.y;
+                        par.v[i][0] = y.x; par.v[i][1] = y.y;
+                    }
+                }
+            };
+            auto exponent = [&](const uint32_t (&u)[4][G], uint32_t least) {      // (a NaN, the sign of a token that was not finite, is passed over)
+                __nv_bfloat162 m = __float2bfloat162_rn(0.f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u[i][g])));
+                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaf(15.f, __low2float(m), __high2float(m))));
+                return min(max(top >> 23, least), 254u);
+            };
+            fetch(0, table[quad_of(0) / ps]);
+            if (n_tiles > 1) page = table[quad_of(1) / ps];
+            for (int j = 0; j < n_tiles; ++j) {
+                const uint32_t word = exponent(par.k, kKeyLeast) | exponent(par.v, kValueLeast) << 8 | (uint32_t)(j + 1) << 16;
+                if (j + 1 < n_tiles) fetch(j + 1, page);
+                if (j + 2 < n_tiles) page = table[quad_of(j + 2) / ps];
+                bool read = false;                       // its slot's word has been taken by every warp of the softmax (and so by the unpacking)
+                for (uint32_t i = 0; i < kSpinLimit && !read; ++i)
+                    read = __all_sync(0xffffffffu, lane >= 4 * n_heads || tops_read[lane & 7] > j - kTopRing);
+                if (!read) { attn_give_up(10); failed = 1; break; }
+                if (lane == 0) tops[j % kTopRing] = word;
+            }
+        }
         if (!PACKED && lane < pages_per_tile) page = table[min(k_begin / ps + lane, a.table_width - 1)];
         for (int j = 0; j < (PACKED ? 0 : n_tiles); ++j) {
             const int s = j & 1, sv = j % kVStages;
@@ -324,9 +418,10 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         // ---- MMA issuer --------------------------------------------------------------------------
         // Order: S_A(0) S_B(0), then per key tile j: PV_A(j) S_A(j+1) PV_B(j) S_B(j+1).  The tensor core runs
         // its instructions in the order of issue, so S_x(j+1) overwrites P_x(j) only after PV_x(j) has read it.
-        constexpr uint32_t idesc_s = umma_idesc(kRows, kKeys);                         // Q, K both K-major
-        constexpr uint32_t idesc_o = umma_idesc(kRows, kDim) | (1u << 16);             // P from TMEM, V MN-major
-        bool ok = mbar_wait(&q_full, 0);
+        constexpr uint32_t half_operands = PACKED ? (1u << 7) | (1u << 10) : 0u;       // (the bits that say bfloat16)
+        constexpr uint32_t idesc_s = umma_idesc(kRows, kKeys) & ~half_operands;        // Q, K both K-major
+        constexpr uint32_t idesc_o = (umma_idesc(kRows, kDim) | (1u << 16)) & ~half_operands;         // P from TMEM, V MN-major
+        bool ok = PACKED ? mbar_wait(&q_ready[0], 0) && (n_heads == 1 || mbar_wait(&q_ready[1], 0)) : mbar_wait(&q_full, 0);
         if (!ok) { attn_give_up(2); failed = 1; }
         // Descriptors are built once; inside the loops only constants are added.
         const uint64_t dq[2] = {umma_desc(q_tile[0]), umma_desc(q_tile[1])};
@@ -433,7 +528,9 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 }
             }
         };
-        auto write = [&](const Units& u, unsigned char* tile, bool value) {
+        auto write = [&](const Units& u, unsigned char* tile, uint32_t e8, bool value) {
+            const __nv_bfloat162 d2 = __float2bfloat162_rn(top_down(e8));
+            const uint32_t down = *reinterpret_cast<const uint32_t*>(&d2);
 #pragma unroll
             for (int i = 0; i < kOctets; ++i) {
                 unsigned char* row = tile + (p + kUnpackWarps * i) * 1024 + r * 128;
@@ -441,7 +538,8 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 for (int g = 0; g < G; ++g) {
                     const uint32_t w = value ? __byte_perm(u.w[i][g / 2], u.w[i][G / 2 + g / 2], (g & 1) ? 0x7632 : 0x5410) : u.w[i][g];
                     const int chunk = 4 * g + jj;
-                    *reinterpret_cast<uint4*>(row + (chunk >> 3) * kHalfBytes + (((chunk & 7) ^ r) << 4)) = unpack_word(w, u.par[i][g]);
+                    *reinterpret_cast<uint4*>(row + (chunk >> 3) * kHalfBytes + (((chunk & 7) ^ r) << 4)) =
+                        unpack_word(w, u.par[i][g], down);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the tensor core reads these through the async proxy
@@ -455,17 +553,19 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         fetch(keys, rows, 0);
         for (int j = 0; j < n_tiles; ++j) {
             const int s = j & 1, sv = j % kVStages;
+            uint32_t word;
             fetch(values, rows, value_at);
             if (j + 1 < n_tiles) look_up(j + 1, page, off);
             if (j >= 2 && !mbar_wait_all(&k_empty[s], ((j >> 1) - 1) & 1)) { attn_give_up(1); failed = 1; break; }
-            write(keys, k_tile[s], false);
+            if (!__all_sync(0xffffffffu, top_wait(tops, j, word))) { attn_give_up(10); failed = 1; break; }
+            write(keys, k_tile[s], top_keys(word), false);
             if (lane == 0) mbar_arrive(&k_full[s]);
             if (j + 1 < n_tiles) {
                 find(rows, j + 1, page, off);
                 fetch(keys, rows, 0);
             }
             if (j >= kVStages && !mbar_wait_all(&v_empty[sv], ((j / kVStages) - 1) & 1)) { attn_give_up(1); failed = 1; break; }
-            write(values, v_tile[sv], true);
+            write(values, v_tile[sv], top_values(word), true);
             if (lane == 0) mbar_arrive(&v_full[sv]);
         }
     } else if (warp >= 2 && ((warp - 2) >> 2) < n_heads) {
@@ -479,10 +579,52 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const int row_lo = a.window > 0 ? row_pos - a.window + 1 : 0;
         float m = -INFINITY, l = 0.f;                  // reference maximum (log2 units) and sum relative to it
         bool ok = true;
-        for (int j = 0; j < n_tiles; ++j) {
+        float sl = a.sl, sl_row = a.sl;                 // of a tile's scores; of this row, over keys as they are
+        if constexpr (PACKED) {
+            // this thread's row of the queries becomes float16, over the power of two of its largest number
+            if (!mbar_wait_all(&q_full, 0)) {
+                attn_give_up(2); failed = 1; ok = false;
+            } else {
+                unsigned char* mine = q_tile[x] + row * 128;
+                uint32_t top = 0u;
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(mine + (c >> 3) * kHalfBytes + (((c & 7) ^ (row & 7)) << 4));
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = max(top, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
+                }
+                const uint32_t e8 = min(max(top >> 23, 1u), 253u);             // (NaN and infinity stay what they are)
+                const float down = __uint_as_float((254u - e8) << 23);
+                sl_row *= __uint_as_float(e8 << 23);
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    uint4* at = reinterpret_cast<uint4*>(mine + (c >> 3) * kHalfBytes + (((c & 7) ^ (row & 7)) << 4));
+                    const uint4 v = *at;
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    uint32_t h[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        h[e] = pack_operand<true>(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xffff0000u) * down);
+                    *at = make_uint4(h[0], h[1], h[2], h[3]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the tensor core reads the tile through the async proxy
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_ready[x]);
+            }
+        }
+        for (int j = 0; j < n_tiles && ok; ++j) {
             if (!mbar_wait(&s_full[x], j & 1)) { attn_give_up(6); failed = 1; ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int t0 = k_begin + j * kKeys;
+            float e = 0.f;                                       // the tile's values are over 2^e
+            if constexpr (PACKED) {
+                uint32_t word;
+                if (!__all_sync(0xffffffffu, top_wait(tops, j, word))) { attn_give_up(10); failed = 1; ok = false; break; }
+                if (lane == 0) tops_read[warp - 2] = j + 1;
+                sl = sl_row * top_up(top_keys(word));
+                e = (float)((int)top_values(word) - 141);
+            }
             const bool need_mask = (t0 + kKeys - 1 > pos0) || (a.window > 0 && t0 < pos_last - a.window + 1);
             uint32_t ca[32], cb[32];
             float sums[4] = {0.f, 0.f, 0.f, 0.f};
@@ -490,7 +632,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             // pass.  P is taken relative to the reference as it stands while the tile's maximum is taken on the way; only
             // if that maximum turns out more than the step above some row's reference (rare after the first tiles) are
             // the tile's P, the row's O and its sum scaled down afterwards, by a whole power of two (exact in bfloat16).
-            if (a.one_pass && j > 0 && !need_mask && __all_sync(0xffffffffu, m != -INFINITY)) {
+            if (!PACKED && a.one_pass && j > 0 && !need_mask && __all_sync(0xffffffffu, m != -INFINITY)) {
                 float mx = -INFINITY;
                 uint32_t packed[16];
                 tmem_ld32(s_addr, ca);
@@ -499,16 +641,16 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     tmem_ld32(s_addr + c0 + 32, cb);
                     mx = chunk_max<false>(ca, t0 + c0, row_pos, row_lo, mx);
-                    chunk_exp<false>(ca, packed, a.sl, m, t0 + c0, row_pos, row_lo, sums);
+                    chunk_exp<false, PACKED>(ca, packed, sl, m, t0 + c0, row_pos, row_lo, sums);
                     tmem_st16(s_addr + (c0 >> 1), packed);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (c0 + 64 < kKeys) tmem_ld32(s_addr + c0 + 64, ca);
                     mx = chunk_max<false>(cb, t0 + c0 + 32, row_pos, row_lo, mx);
-                    chunk_exp<false>(cb, packed, a.sl, m, t0 + c0 + 32, row_pos, row_lo, sums);
+                    chunk_exp<false, PACKED>(cb, packed, sl, m, t0 + c0 + 32, row_pos, row_lo, sums);
                     tmem_st16(s_addr + (c0 >> 1) + 16, packed);
                 }
                 float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-                const float grown = mx * a.sl - m;
+                const float grown = mx * sl - m;
                 if (__any_sync(0xffffffffu, grown > kRescaleStep)) {
                     // beyond this the exponentials above may have left float32's range: the result is void, and said to be
                     if (grown > kOnePassLimit) attn_give_up(9);
@@ -561,7 +703,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             const float mx = need_mask ? pass_max(std::true_type{}) : pass_max(std::false_type{});
             tmem_ld32(s_addr, ca);                                   // pass 2's first chunk, in flight during the decision
             // move the reference only when the maximum has grown by more than the step (always from -inf)
-            const float m_tile = mx * a.sl;
+            const float m_tile = mx * sl + e;
             const bool move = m_tile > m + kRescaleStep || (m == -INFINITY && m_tile > -INFINITY);
             if (j > 0 && __any_sync(0xffffffffu, move)) {
                 // O of the tiles so far is complete (the scores of this tile were issued after their P V): its rows are scaled
@@ -578,7 +720,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 l *= f;
             }
             if (move) m = m_tile;
-            const float mu = m == -INFINITY ? 0.f : m;      // a row with no visible key yet
+            const float mu = (m == -INFINITY ? 0.f : m) - (PACKED ? e + kPackedP : 0.f);      // (a row with no visible key yet: any reference)
             auto pass_exp = [&](auto tag) {
                 constexpr bool MASK = decltype(tag)::value;
                 uint32_t packed[16];
@@ -586,17 +728,17 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 for (int c0 = 0; c0 < kKeys; c0 += 64) {
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     tmem_ld32(s_addr + c0 + 32, cb);
-                    chunk_exp<MASK>(ca, packed, a.sl, mu, t0 + c0, row_pos, row_lo, sums);
+                    chunk_exp<MASK, PACKED>(ca, packed, sl, mu, t0 + c0, row_pos, row_lo, sums);
                     tmem_st16(s_addr + (c0 >> 1), packed);           // keys c0 .. c0+31 as 16 columns of two bfloat16
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (c0 + 64 < kKeys) tmem_ld32(s_addr + c0 + 64, ca);
-                    chunk_exp<MASK>(cb, packed, a.sl, mu, t0 + c0 + 32, row_pos, row_lo, sums);
+                    chunk_exp<MASK, PACKED>(cb, packed, sl, mu, t0 + c0 + 32, row_pos, row_lo, sums);
                     tmem_st16(s_addr + (c0 >> 1) + 16, packed);
                 }
             };
             if (need_mask) pass_exp(std::true_type{}); else pass_exp(std::false_type{});
             const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-            l += sum;
+            l += PACKED ? sum * ex2(-e) : sum;
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
