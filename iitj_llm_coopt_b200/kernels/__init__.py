@@ -901,6 +901,7 @@ class Kernels:
         _need(heads > 0 and heads % kv_heads == 0, f"attention_kv4: heads {heads} is not a multiple of kv_heads {kv_heads}")
         _need(q.shape[1] >= heads * head_dim, "attention_kv4.q: row too narrow")
         _need(out.shape == (tokens, heads * head_dim), "attention_kv4.out: wrong shape")
+        _need(0.0 <= scale < math.inf, f"attention_kv4: scale {scale}: a positive number, or 0 for 1 / sqrt(head_dim)")
         _check(meta.block_table, "attention_kv4.block_table", torch.int32, 2)
         _check(meta.token_request, "attention_kv4.token_request", torch.int32, 1)
         _check(meta.positions, "attention_kv4.positions", torch.int32, 1)

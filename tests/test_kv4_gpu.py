@@ -220,6 +220,34 @@ def test_large_scores_and_a_scale_of_its_own(K, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 200])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("keys,late_keys,values,late_values", [(2.0 ** -60, 1, 2.0 ** -25, 1), (2.0 ** 70, 1, 2.0 ** 50, 1),
+                                                               (1, 2.0 ** -16, 2.0 ** -16, 2.0 ** 16), (2.0 ** -16, 2.0 ** 16, 1, 2.0 ** -16),
+                                                               (1, 1, 0.0, 1), (0.0, 1, 1, 0.0), (1, 1, 2.0 ** 20, 0.0)])
+def test_small_and_large_numbers(K, dtype, new, D, keys, late_keys, values, late_values):
+    """Keys and values times powers of two, those from token 150 on times others yet; queries that bring the scores back to where
+    they were.  (1600 keys: the kernels' splits too.)"""
+    lens, news, page = [200, 1600], [new, new], 16
+    q, cache, table, meta = case(12, lens, news, 4, 2, D, page, dtype, spoil=False)
+    for b, n in enumerate(lens):
+        p = torch.arange(n)
+        late = (p >= 150)[:, None, None]
+        k, v = rnd(n, 2, D, seed=1200 + b), rnd(n, 2, D, seed=1250 + b)
+        k, v = k * torch.where(late, late_keys, 1.0) * keys, v * torch.where(late, late_values, 1.0) * (values or 1.0)
+        if not values:
+            v[:150] = 0.0
+        P.store(cache, table[b].long()[p // page] * page + p % page, k.to(dtype), v.to(dtype), page)
+    q = q / (max(keys, keys * late_keys) or 1.0)
+    want, tol = P.attend(q, cache, table, lens, news, 4, 2, page, D, unit=P.U16 if dtype == torch.bfloat16 else P.U32)
+    out = torch.full((q.shape[0], 4 * D), 7.0, dtype=dtype, device="cuda")
+    K.attention_kv4(q.cuda(), cache.cuda(), meta, out, 4, 2, D)
+    K.check_health()
+    got = out.cpu().double()
+    assert bool(got.isfinite().all()) and bool(((got - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("new", [1, 130])
 def test_a_token_that_is_not_finite_reaches_only_those_who_see_it(K, dtype, new):
     """A key of NaN at position 150 of 200: queries before it give what they give without it, queries behind it NaN."""
@@ -359,7 +387,8 @@ def test_refusals(K):
     good = dict(q=z(3, 256), cache_layer=cache, meta=meta, out=z(3, 256), heads=4, kv_heads=2, head_dim=64)
     for bad, text in ((dict(heads=5), "multiple of kv_heads"), (dict(out=z(3, 128)), "out"), (dict(q=z(3, 128)), "narrow"),
                       (dict(out=z(3, 256, t=torch.float32)), "dtype"), (dict(cache_layer=cache[:, 16:]), "contiguous"),
-                      (dict(q=z(2, 256), out=z(2, 256)), "one position per token")):
+                      (dict(q=z(2, 256), out=z(2, 256)), "one position per token"),
+                      (dict(scale=-0.1), "positive"), (dict(scale=math.nan), "positive"), (dict(scale=math.inf), "positive")):
         with pytest.raises(KernelError, match=text):
             K.attention_kv4(**{**good, **bad})
     pool = z(2, 6, 32)
