@@ -35,7 +35,6 @@
 //   values   over such a power 2^e as well.  P of the tile is taken times 2^e, so O needs nothing; l takes it back.  The reference
 //            M follows the scores plus e: what float16 flushes lies 2^-29 below the tile's largest value, or 2^-32 below the row's
 //            largest product
-// P must not pass float16's range before its row's reference moves, so every tile takes the two passes over its scores.
 //
 // Every mbarrier wait is bounded; a wait that runs out records a code (llm_attention_tcgen05_status)
 // and the CTA falls through to its teardown, where the tensor memory is freed.
@@ -379,9 +378,9 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 const uint32_t word = exponent(par.k, kKeyLeast) | exponent(par.v, kValueLeast) << 8 | (uint32_t)(j + 1) << 16;
                 if (j + 1 < n_tiles) fetch(j + 1, page);
                 if (j + 2 < n_tiles) page = table[quad_of(j + 2) / ps];
-                bool read = false;                       // its slot's word has been taken by every warp of the softmax (and so by the unpacking)
+                bool read = false;                       // its slot's word has been taken by the softmax (the one behind it: by the unpacking too)
                 for (uint32_t i = 0; i < kSpinLimit && !read; ++i)
-                    read = __all_sync(0xffffffffu, lane >= 4 * n_heads || tops_read[lane & 7] > j - kTopRing);
+                    read = __all_sync(0xffffffffu, lane >= 4 * n_heads || tops_read[lane & 7] > j + 1 - kTopRing);
                 if (!read) { attn_give_up(10); failed = 1; break; }
                 if (lane == 0) tops[j % kTopRing] = word;
             }
@@ -488,7 +487,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const size_t page_bytes = (size_t)a.kv_heads * block_bytes;
         const int page_shift = (ps & (ps - 1)) ? -1 : 31 - __clz(ps), value_at = ps * 20 * G, par_at = ps * 16 * G;
         struct Units { uint32_t w[kOctets][G], par[kOctets][G]; };
-        struct Rows { const uint8_t* codes[kOctets]; const uint8_t* par[kOctets]; };
+        struct Rows { const uint8_t* codes[kOctets]; int to_par[kOctets]; };
         // Lane x looks up the page of keys 4 x .. 4 x + 3 of a tile (they share one), and the first one's place in it.  Keys outside the
         // rows' reach are taken from its ends: nothing behind a request's last token, or in a page given back, is read.
         auto look_up = [&](int j, int& page, int& off) {
@@ -510,13 +509,13 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 }
                 const uint8_t* page_at = cache + (size_t)__shfl_sync(0xffffffffu, page, from) * page_bytes;
                 rows.codes[i] = page_at + at * 16 * G + 4 * G * jj;
-                rows.par[i] = page_at + par_at + at * 4 * G;
+                rows.to_par[i] = par_at - at * 12 * G - 4 * G * jj;
             }
         };
         auto fetch = [&](Units& u, const Rows& rows, int region) {            // region: 0, or value_at
 #pragma unroll
             for (int i = 0; i < kOctets; ++i) {
-                const uint8_t *codes = rows.codes[i] + region, *par = rows.par[i] + region;
+                const uint8_t *codes = rows.codes[i] + region, *par = codes + rows.to_par[i];
                 if constexpr (G == 4) {
                     const uint4 c = *reinterpret_cast<const uint4*>(codes), q = *reinterpret_cast<const uint4*>(par);
                     u.w[i][0] = c.x; u.w[i][1] = c.y; u.w[i][2] = c.z; u.w[i][3] = c.w;
@@ -614,9 +613,6 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             }
         }
         for (int j = 0; j < n_tiles && ok; ++j) {
-            if (!mbar_wait(&s_full[x], j & 1)) { attn_give_up(6); failed = 1; ok = false; break; }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const int t0 = k_begin + j * kKeys;
             float e = 0.f;                                       // the tile's values are over 2^e
             if constexpr (PACKED) {
                 uint32_t word;
@@ -625,6 +621,9 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 sl = sl_row * top_up(top_keys(word));
                 e = (float)((int)top_values(word) - 141);
             }
+            if (!mbar_wait(&s_full[x], j & 1)) { attn_give_up(6); failed = 1; ok = false; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int t0 = k_begin + j * kKeys;
             const bool need_mask = (t0 + kKeys - 1 > pos0) || (a.window > 0 && t0 < pos_last - a.window + 1);
             uint32_t ca[32], cb[32];
             float sums[4] = {0.f, 0.f, 0.f, 0.f};
@@ -632,7 +631,59 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             // pass.  P is taken relative to the reference as it stands while the tile's maximum is taken on the way; only
             // if that maximum turns out more than the step above some row's reference (rare after the first tiles) are
             // the tile's P, the row's O and its sum scaled down afterwards, by a whole power of two (exact in bfloat16).
-            if (!PACKED && a.one_pass && j > 0 && !need_mask && __all_sync(0xffffffffu, m != -INFINITY)) {
+            // Float16 would not hold P before the reference has moved: over a packed cache the maximum of half a tile comes first, from
+            // the registers that its P is made of (without that, the two passes: 709 us against 651 over 8192 tokens, 32 heads).
+            const bool whole = j > 0 && !need_mask && __all_sync(0xffffffffu, m != -INFINITY);
+            if (PACKED && whole) {
+                uint32_t packed[16];
+                tmem_ld32(s_addr, ca);
+                tmem_ld32(s_addr + 32, cb);
+#pragma unroll 1
+                for (int c0 = 0; c0 < kKeys; c0 += 64) {
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    const float mx = fmaxf(chunk_max<false>(ca, t0 + c0, row_pos, row_lo, -INFINITY),
+                                           chunk_max<false>(cb, t0 + c0 + 32, row_pos, row_lo, -INFINITY));
+                    const float grown = mx * sl + e - m;
+                    if (__any_sync(0xffffffffu, grown > kRescaleStep)) {
+                        const float k = grown > kRescaleStep ? ceilf(grown) : 0.f, f = k > 126.f ? 0.f : __int_as_float((127 - (int)k) << 23);
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");   // P is read back below
+                        // (O of the tiles so far is complete: the scores of this tile were issued after their P V)
+#pragma unroll 1
+                        for (int c = 0; c < kDim; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o_addr + c, o);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st16(o_addr + c, o);
+                        }
+#pragma unroll 1
+                        for (int c = 0; c < c0 / 2; c += 16) {
+                            uint32_t pp[16];
+                            tmem_ld16(s_addr + c, pp);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&pp[i]));
+                                pp[i] = pack_operand<true>(v.x * f, v.y * f);
+                            }
+                            tmem_st16(s_addr + c, pp);
+                        }
+                        l *= f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sums[i] *= f;
+                        m += k;
+                    }
+                    const float mu = m - (e + kPackedP);
+                    chunk_exp<false, PACKED>(ca, packed, sl, mu, t0 + c0, row_pos, row_lo, sums);
+                    tmem_st16(s_addr + (c0 >> 1), packed);
+                    if (c0 + 64 < kKeys) tmem_ld32(s_addr + c0 + 64, ca);
+                    chunk_exp<false, PACKED>(cb, packed, sl, mu, t0 + c0 + 32, row_pos, row_lo, sums);
+                    tmem_st16(s_addr + (c0 >> 1) + 16, packed);
+                    if (c0 + 64 < kKeys) tmem_ld32(s_addr + c0 + 96, cb);
+                }
+                l += ((sums[0] + sums[1]) + (sums[2] + sums[3])) * __int_as_float((127 - (int)e) << 23);
+            } else if (!PACKED && a.one_pass && j > 0 && !need_mask && __all_sync(0xffffffffu, m != -INFINITY)) {
                 float mx = -INFINITY;
                 uint32_t packed[16];
                 tmem_ld32(s_addr, ca);
@@ -738,7 +789,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             };
             if (need_mask) pass_exp(std::true_type{}); else pass_exp(std::false_type{});
             const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-            l += PACKED ? sum * ex2(-e) : sum;
+            l += PACKED ? sum * __int_as_float((127 - (int)e) << 23) : sum;
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
