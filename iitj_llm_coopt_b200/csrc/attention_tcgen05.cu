@@ -35,6 +35,9 @@
 //   values   over such a power 2^e as well.  P of the tile is taken times 2^e, so O needs nothing; l takes it back.  The reference
 //            M follows the scores plus e: what float16 flushes lies 2^-29 below the tile's largest value, or 2^-32 below the row's
 //            largest product
+// Measured, 32 heads over 8 of 128 numbers: a prompt of 2048 tokens 62.7 us (over a bfloat16 cache 47), of 8192 tokens 651 us, 845
+// TFLOP/s (492 to 530).  Unpacking does not bound it: with the codes left as they are it took as long.  What it has more than the other form
+// is the maximum before the probabilities, the exponents, and registers: 14 warps leave a thread 128.
 //
 // Every mbarrier wait is bounded; a wait that runs out records a code (llm_attention_tcgen05_status)
 // and the CTA falls through to its teardown, where the tensor memory is freed.

