@@ -963,16 +963,14 @@ class Kernels:
             first = np.maximum(pos - window + 1, 0) if window > 0 else np.zeros_like(pos)
             spans = pos // tile - first // tile + 1
             pairs, longest = kv_heads * -(-(heads // kv_heads) // 8), int(spans.max())
-            best = None
-            for n in range(1, max(1, -(-longest // warps)) + 1):
-                per = -(-longest // (n * warps)) * warps
-                blocks = int((-(-spans // per)).sum()) * pairs
-                cost = -(-blocks // slots) * (self.KV4_BLOCK + per // warps) + (self.KV4_JOIN if longest > per else 0.0)
-                if best is None or cost < best[0]:
-                    best = (cost, per)
-                if blocks > 4 * slots:
-                    break
-            plan._splits[key] = (best[1], -(-longest // best[1]))
+            # every number of tiles that some count of equal splits comes to, the largest first, up to four rounds of blocks
+            per = -np.unique(-(-(-longest // (np.arange(1, max(1, -(-longest // warps)) + 1) * warps)) * warps))
+            if len(spans) * pairs > 4 * slots:
+                per = per[:1]
+            blocks = (-(-spans // per[:, None])).sum(axis=1) * pairs
+            cost = -(-blocks // slots) * (self.KV4_BLOCK + per // warps) + np.where(per < longest, self.KV4_JOIN, 0.0)
+            per = int(per[np.argmin(cost[:1 + int((blocks <= 4 * slots).sum())])])
+            plan._splits[key] = (per, -(-longest // per))
         return plan._splits[key]
 
     # Costs of `kv4_splits`, in the time that a block's warps take for a tile each: a block's start and end, the second kernel.

@@ -248,6 +248,21 @@ def test_small_and_large_numbers(K, dtype, new, D, keys, late_keys, values, late
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("news", [[1, 1], [290, 150]])
+def test_queries_of_zeros_and_of_the_smallest_numbers(K, dtype, window, news):
+    """Scores of 0: the mean of the values that the window shows."""
+    q, cache, table, meta = case(13, [290, 150], news, 4, 2, 64, 16, dtype)
+    q[::2] = 0.0
+    q[1::4] *= 1e-38
+    want, tol = P.attend(q, cache, table, [290, 150], news, 4, 2, 16, 64, window, 0.0, P.U16 if dtype == torch.bfloat16 else P.U32)
+    out = torch.full((q.shape[0], 256), 7.0, dtype=dtype, device="cuda")
+    K.attention_kv4(q.cuda(), cache.cuda(), meta, out, 4, 2, 64, window=window)
+    K.check_health()
+    assert bool(((out.cpu().double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("new", [1, 130])
 def test_a_token_that_is_not_finite_reaches_only_those_who_see_it(K, dtype, new):
     """A key of NaN at position 150 of 200: queries before it give what they give without it, queries behind it NaN."""
