@@ -96,7 +96,7 @@ class RotaryEmbedding(Part):
         return tabs
 
     def encode_and_store(self, ctx, qkv, cache_view, slots, heads, kv_heads):
-        if cache_view.dtype == torch.uint8:            # a packed cache
+        if cache_view is not None and cache_view.dtype == torch.uint8:            # a packed cache
             return self.k.rope_store_kv4(qkv, self.tables(ctx) if self.rotary_dim else None, slots, cache_view, heads, kv_heads,
                                          self.head_dim, self.rotary_dim)
         return self.k.rope_store(qkv, ctx.positions, self.inv_freq, slots, cache_view, heads, kv_heads,
