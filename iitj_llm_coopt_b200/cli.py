@@ -11,7 +11,7 @@ Options keep the reference's names and meanings where it has them: the client's 
 (bench/run.py:262-274) and the server's --model, --max-num-seqs (256), --max-num-batched-tokens (2048), --kv-gb,
 --max-model-len (32768), --gpu-memory-utilization (0.9), --dtype (engine/server.py:173-201).  There is no HTTP: the
 requests go straight into the engine.  In place of a model folder, `--shape NAME --random-seed S` builds a model of
-a named shape (presets.py) with random weights.
+a named shape (presets.py) with random weights.  `--kv-cache int4` keeps keys and values as 4-bit codes.
 
 Workloads:
   FILE.jsonl                       one JSON object per line with `prompt_token_ids` and `max_tokens` (optionally `id`,
