@@ -450,6 +450,7 @@ class Kernels:
         self._scratch_bufs: dict = {}
         self._pair_counters: dict = {}
         self._kv4_pages: dict = {}       # (bytes of a page, kv_heads, head_dim) -> tokens of a packed page
+        self._kv4_sizes: set = set()     # (width of a row, heads, kv_heads, head_dim, rotary_dim) of rope_store_kv4 that were found good
         self._kv4_forms: dict = {}       # (heads, kv_heads, head_dim, page size) -> whether the packed prompt and single-token kernels take it
         self._linear_plans: dict = {}    # (tokens, n, k, swiglu) -> (kernel, k-splits, shared memory, half-tile form)
         self.scratch_generation = 0
@@ -723,8 +724,21 @@ class Kernels:
             _need(kv_heads > 0 and cache_layer.shape[1] % (4 * token) == 0 and cache_layer.shape[1] > 0,
                   f"{name}.cache: pages of {cache_layer.shape[1]} bytes are no multiple of 4 tokens of {kv_heads} heads of {head_dim} numbers")
             page_size = self._kv4_pages[key] = cache_layer.shape[1] // token
-        _need(cache_layer.data_ptr() % 16 == 0, f"{name}.cache: not on a 16-byte boundary")
         return page_size
+
+    @staticmethod
+    def _aligned(name, **tensors):
+        """Raises for the first tensor that is not on a 16-byte boundary."""
+        for what, t in tensors.items():
+            _need(t is None or t.data_ptr() % 16 == 0, f"{name}.{what}: not on a 16-byte boundary")
+
+    def _rope_kv4_sizes(self, width, heads, kv_heads, head_dim, rotary_dim):
+        """Checks the sizes of a `rope_store_kv4`, once for each set of them."""
+        _need(heads > 0 and kv_heads > 0 and width == (heads + 2 * kv_heads) * head_dim,
+              "rope_store_kv4.qkv: width is not (heads+2*kv_heads)*head_dim")
+        _need(0 <= rotary_dim <= head_dim and rotary_dim % 16 == 0, f"rope_store_kv4: rotary_dim {rotary_dim} is not a multiple of 16 up to {head_dim}")
+        _need(head_dim % 32 == 0 and 32 <= head_dim <= 256, f"rope_store_kv4: head_dim {head_dim} is not a multiple of 32 up to 256")
+        self._kv4_sizes.add((width, heads, kv_heads, head_dim, rotary_dim))
 
     def rope_store_kv4(self, qkv, tables, slots, cache_layer, heads, kv_heads, head_dim, rotary_dim, q_out=None):
         """`rope_store` into a packed cache: rotates the queries, rotates and packs the keys, packs the values and stores both in
@@ -742,10 +756,8 @@ class Kernels:
                 qkv = qkv.sum()
         _check(qkv, "rope_store_kv4.qkv", tuple(DTYPE_CODE), 2)
         tokens = qkv.shape[0]
-        _need(heads > 0 and kv_heads > 0 and qkv.shape[1] == (heads + 2 * kv_heads) * head_dim,
-              "rope_store_kv4.qkv: width is not (heads+2*kv_heads)*head_dim")
-        _need(0 <= rotary_dim <= head_dim and rotary_dim % 16 == 0, f"rope_store_kv4: rotary_dim {rotary_dim} is not a multiple of 16 up to {head_dim}")
-        _need(head_dim % 32 == 0 and 32 <= head_dim <= 256, f"rope_store_kv4: head_dim {head_dim} is not a multiple of 32 up to 256")
+        if (qkv.shape[1], heads, kv_heads, head_dim, rotary_dim) not in self._kv4_sizes:
+            self._rope_kv4_sizes(qkv.shape[1], heads, kv_heads, head_dim, rotary_dim)
         cos = sin = None
         if rotary_dim:
             _need(tables is not None, "rope_store_kv4: a rotation needs its tables")
@@ -763,12 +775,14 @@ class Kernels:
             _need(q_out.shape == (tokens, heads * head_dim), "rope_store_kv4.q_out: wrong shape")
         else:
             q_out = qkv
-        for name, t in (("qkv", qkv), ("q_out", q_out), ("cos", cos), ("sin", sin)):
-            _need(t is None or t.data_ptr() % 16 == 0, f"rope_store_kv4.{name}: not on a 16-byte boundary")
-        self._call("llm_rope_store_kv4", None if parts is not None else _ptr(qkv), _ptr(parts.parts) if parts is not None else None,
-                   parts.splits if parts is not None else 0, parts.stride if parts is not None else 0, _ptr(q_out), q_out.shape[1],
-                   _ptr(cos), _ptr(sin), _ptr(slots), _ptr(cache_layer) if slots is not None else None, DTYPE_CODE[qkv.dtype], tokens,
-                   heads, kv_heads, head_dim, rotary_dim, page_size, self._stream())
+        at, q_at, cos_at, sin_at = qkv.data_ptr(), q_out.data_ptr(), _ptr(cos), _ptr(sin)
+        cache_at = cache_layer.data_ptr() if slots is not None else None
+        if (at | q_at | (cos_at or 0) | (sin_at or 0) | (cache_at or 0)) & 15:
+            self._aligned("rope_store_kv4", qkv=qkv, q_out=q_out, cos=cos, sin=sin, cache=cache_layer)
+        parts_at = parts.parts.data_ptr() if parts is not None else None
+        self._call("llm_rope_store_kv4", None if parts_at is not None else at, parts_at, parts.splits if parts is not None else 0,
+                   parts.stride if parts is not None else 0, q_at, q_out.shape[1], cos_at, sin_at, _ptr(slots), cache_at,
+                   DTYPE_CODE[qkv.dtype], tokens, heads, kv_heads, head_dim, rotary_dim, page_size, self._stream())
         return q_out
 
     def kv4_read(self, cache_layer, slots, out, kv_heads, head_dim):
@@ -777,9 +791,11 @@ class Kernels:
         page_size = self._kv4_page_size("kv4_read", cache_layer, kv_heads, head_dim)
         _check(slots, "kv4_read.slots", torch.int32, 1)
         _check(out, "kv4_read.out", tuple(DTYPE_CODE), 4)
-        _need(tuple(out.shape) == (slots.shape[0], 2, kv_heads, head_dim), "kv4_read.out: wrong shape")
-        _need(out.data_ptr() % 16 == 0, "kv4_read.out: not on a 16-byte boundary")
-        self._call("llm_kv4_read", _ptr(cache_layer), _ptr(slots), _ptr(out), DTYPE_CODE[out.dtype], slots.shape[0], kv_heads, head_dim,
+        _need(out.shape == (slots.shape[0], 2, kv_heads, head_dim), "kv4_read.out: wrong shape")
+        cache_at, out_at = cache_layer.data_ptr(), out.data_ptr()
+        if (cache_at | out_at) & 15:
+            self._aligned("kv4_read", cache=cache_layer, out=out)
+        self._call("llm_kv4_read", cache_at, slots.data_ptr(), out_at, DTYPE_CODE[out.dtype], slots.shape[0], kv_heads, head_dim,
                    page_size, self._stream())
         return out
 
@@ -896,26 +912,31 @@ class Kernels:
         heads first in each row) over the numbers that its request's codes stand for."""
         _check(q, "attention_kv4.q", tuple(DTYPE_CODE), 2)
         _check(out, "attention_kv4.out", q.dtype, 2)
-        tokens = q.shape[0]
+        tokens, width = q.shape
         page_size = self._kv4_page_size("attention_kv4", cache_layer, kv_heads, head_dim)
-        _need(heads > 0 and heads % kv_heads == 0, f"attention_kv4: heads {heads} is not a multiple of kv_heads {kv_heads}")
-        _need(q.shape[1] >= heads * head_dim, "attention_kv4.q: row too narrow")
+        if heads <= 0 or heads % kv_heads:
+            raise KernelError(f"attention_kv4: heads {heads} is not a multiple of kv_heads {kv_heads}")
+        _need(width >= heads * head_dim, "attention_kv4.q: row too narrow")
         _need(out.shape == (tokens, heads * head_dim), "attention_kv4.out: wrong shape")
-        _need(0.0 <= scale < math.inf, f"attention_kv4: scale {scale}: a positive number, or 0 for 1 / sqrt(head_dim)")
-        _check(meta.block_table, "attention_kv4.block_table", torch.int32, 2)
-        _check(meta.token_request, "attention_kv4.token_request", torch.int32, 1)
-        _check(meta.positions, "attention_kv4.positions", torch.int32, 1)
-        _need(meta.token_request.shape[0] == tokens and meta.positions.shape[0] == tokens,
-              "attention_kv4: one token_request and one position per token")
-        if not scale:
-            scale = 1.0 / math.sqrt(head_dim)
+        if not 0.0 <= scale < math.inf:
+            raise KernelError(f"attention_kv4: scale {scale}: a positive number, or 0 for 1 / sqrt(head_dim)")
+        block_table, request, positions = meta.block_table, meta.token_request, meta.positions
+        _check(block_table, "attention_kv4.block_table", torch.int32, 2)
+        _check(request, "attention_kv4.token_request", torch.int32, 1)
+        _check(positions, "attention_kv4.positions", torch.int32, 1)
+        _need(request.shape[0] == tokens and positions.shape[0] == tokens, "attention_kv4: one token_request and one position per token")
+        q_at, out_at, cache_at = q.data_ptr(), out.data_ptr(), cache_layer.data_ptr()
+        if cache_at & 15:
+            self._aligned("attention_kv4", cache=cache_layer)
+        scale = float(scale) if scale else 1.0 / math.sqrt(head_dim)
         if not tokens:
             return out
+        table = (cache_at, block_table.data_ptr(), block_table.shape[1])
+        shape = (heads, kv_heads, head_dim, page_size)
         # the fast forms: of the prompt portions (bfloat16 on tcgen05, float32 by query tiles), of the single tokens (bfloat16)
         plan, portions, singles = None, False, False
-        if getattr(meta, "query_lens", None) is not None and q.data_ptr() % 16 == 0 and q.shape[1] % 8 == 0 and out.data_ptr() % 16 == 0:
+        if getattr(meta, "query_lens", None) is not None and not (q_at | out_at) & 15 and width % 8 == 0:
             plan = attention_plan(meta, q.device)
-            shape = (heads, kv_heads, head_dim, page_size)
             forms = self._kv4_forms.get(shape)
             if forms is None:
                 forms = self._kv4_forms[shape] = (self.lib.llm_attention_kv4_prompt_supported(*shape), self.lib.llm_attention_kv4_single_supported(*shape))
@@ -923,22 +944,21 @@ class Kernels:
         rows, n_rows = None, tokens           # what is left to the general kernel
         if plan is not None and (portions or not plan.n_tiles):
             if plan.n_tiles and q.dtype == torch.bfloat16:
-                self._kv4_prompt(q, cache_layer, meta, plan, out, *shape, int(window), float(scale))
+                self._kv4_prompt(q, table, plan, out, shape, int(window), scale)
             elif plan.n_tiles:
-                self._call("llm_attention_kv4_f32_tiles", _ptr(q), q.shape[1], _ptr(cache_layer), _ptr(meta.block_table), meta.block_table.shape[1],
-                           _ptr(plan.tiles), plan.n_tiles, _ptr(out), out.shape[1], heads, kv_heads, head_dim, page_size, int(window),
-                           float(scale), self._stream())
+                self._call("llm_attention_kv4_f32_tiles", q_at, width, *table, _ptr(plan.tiles), plan.n_tiles, out_at, out.shape[1], *shape,
+                           int(window), scale, self._stream())
             rows, n_rows = plan.items, plan.n_items
             if n_rows and singles:
-                self._kv4_single(q, cache_layer, meta, plan, out, *shape, int(window), float(scale))
+                self._kv4_single(q, table, request, positions, plan, out, shape, int(window), scale)
                 n_rows = 0
         if n_rows:
-            self._call("llm_attention_kv4_general", _ptr(q), q.shape[1], _ptr(cache_layer), _ptr(meta.block_table), meta.block_table.shape[1],
-                       _ptr(rows), n_rows, _ptr(meta.token_request), _ptr(meta.positions), _ptr(out), out.shape[1], DTYPE_CODE[q.dtype],
-                       heads, kv_heads, head_dim, page_size, int(window), float(scale), self._stream())
+            self._call("llm_attention_kv4_general", q_at, width, *table, _ptr(rows), n_rows, request.data_ptr(), positions.data_ptr(), out_at,
+                       out.shape[1], DTYPE_CODE[q.dtype], *shape, int(window), scale, self._stream())
         return out
 
-    def _kv4_prompt(self, q, cache_layer, meta, plan, out, heads, kv_heads, head_dim, page_size, window, scale):
+    def _kv4_prompt(self, q, table, plan, out, shape, window, scale):
+        heads, kv_heads, head_dim, _page_size = shape
         if plan.big_tiles is None:
             plan.big_tiles = torch.tensor(plan.big_rows, dtype=torch.int32).to(q.device)
         splits = self.prefill_key_splits(plan.big_rows, heads, kv_heads, window)
@@ -948,9 +968,8 @@ class Kernels:
             part_o = torch.empty(n * head_dim, dtype=torch.float32, device=q.device)
             part_ml = torch.empty(n * 2, dtype=torch.float32, device=q.device)
             self.launches += 1
-        self._call("llm_attention_kv4_prompt", _ptr(q), q.shape[1], q.shape[0], _ptr(cache_layer), _ptr(meta.block_table),
-                   meta.block_table.shape[1], _ptr(plan.big_tiles), len(plan.big_rows), _ptr(out), out.shape[1], heads, kv_heads, head_dim,
-                   page_size, window, scale, splits, _ptr(part_o), _ptr(part_ml), self._stream())
+        self._call("llm_attention_kv4_prompt", q.data_ptr(), q.shape[1], q.shape[0], *table, plan.big_tiles.data_ptr(), len(plan.big_rows),
+                   out.data_ptr(), out.shape[1], *shape, window, scale, splits, _ptr(part_o), _ptr(part_ml), self._stream())
 
     def kv4_splits(self, plan, heads, kv_heads, window) -> tuple:
         """(tiles of 32 keys a block takes, most blocks of any item and head) of a step's single tokens over a packed cache."""
@@ -976,17 +995,19 @@ class Kernels:
     # Costs of `kv4_splits`, in the time that a block's warps take for a tile each: a block's start and end, the second kernel.
     KV4_BLOCK, KV4_JOIN = 2.5, 3.0
 
-    def _kv4_single(self, q, cache_layer, meta, plan, out, heads, kv_heads, head_dim, page_size, window, scale):
+    def _kv4_single(self, q, table, request, positions, plan, out, shape, window, scale):
+        heads, kv_heads, head_dim, _page_size = shape
         tiles, splits = self.kv4_splits(plan, heads, kv_heads, window)
-        part_o = part_ml = None
+        o_at = ml_at = None
         if splits > 1:
             # allocated for the call, not kept: steps on two streams, or of two captured graphs, do not share it
-            part_o = torch.empty(plan.n_items * heads * splits * head_dim, dtype=torch.float32, device=q.device)
-            part_ml = torch.empty(plan.n_items * heads * splits * 2, dtype=torch.float32, device=q.device)
+            n = plan.n_items * heads * splits
+            parts = torch.empty(n * (head_dim + 2), dtype=torch.float32, device=q.device)
+            o_at = parts.data_ptr()
+            ml_at = o_at + n * head_dim * 4
             self.launches += 1
-        self._call("llm_attention_kv4_single", _ptr(q), q.shape[1], _ptr(cache_layer), _ptr(meta.block_table), meta.block_table.shape[1],
-                   _ptr(plan.items), plan.n_items, _ptr(meta.token_request), _ptr(meta.positions), _ptr(part_o), _ptr(part_ml), _ptr(out),
-                   out.shape[1], heads, kv_heads, head_dim, page_size, window, scale, tiles, splits, self._stream())
+        self._call("llm_attention_kv4_single", q.data_ptr(), q.shape[1], *table, plan.items.data_ptr(), plan.n_items, request.data_ptr(),
+                   positions.data_ptr(), o_at, ml_at, out.data_ptr(), out.shape[1], *shape, window, scale, tiles, splits, self._stream())
 
     def _attention_f32_takes(self, qkv, cache_layer, meta, out, heads, kv_heads, head_dim) -> bool:
         """True if float32 attention runs on the tile and single-token kernels: head sizes 64 and 128, rows on 16-byte
