@@ -10,8 +10,8 @@
 // another until the end.  A block takes one split of an item's tiles, dealt out in turn to its warps, and joins their sums; with more
 // than one split the blocks leave theirs in scratch memory, and a second kernel joins those.
 //
-// Measured, 32 heads over 8 of 128 numbers: 8 requests over 8192 tokens 29.7 us, 2.8 TB/s of codes (the reading alone would take 12.8);
-// 2 over 32768 tokens 30.7.  What bounds the loop now is the issue of instructions, about 720 a tile of 32 keys and 8 heads, half of
+// Measured, 32 heads over 8 of 128 numbers: 8 requests over 8192 tokens 30.8 us, 2.7 TB/s of codes (the reading alone would take 12.8);
+// 2 over 32768 tokens 31.8.  What bounds the loop now is the issue of instructions, about 720 a tile of 32 keys and 8 heads, half of
 // them integer ones, beside the matrix instructions' own time.
 //
 //   scores   mma m16n8k16, 16 keys x 8 query heads.  A code n becomes the float16 1024 + n or 64 + n by one AND-OR (its last mantissa
@@ -20,10 +20,12 @@
 //            products: one operand are the stored (s, z) words as they lie, the other one the sums of q (as three bfloat16 each).  Nothing
 //            of the key is rounded.
 //   values   the transposed product, 16 numbers x 8 heads over 16 keys: the operand is n - 8 (128 + n - 136, exact), the other one
-//            p s, p rounded to bfloat16 and the product rounded again, a group at a time.  The middles z + 8 s (rounded to bfloat16: they
-//            are small beside the numbers) and the sum of p are one more product, of rows of middles and of ones, with the same p.
+//            p s, rounded once to bfloat16 (float16 would not hold s), a group at a time.  p crosses the lanes as float16, times 2^7 so that
+//            what is flushed lies 2^-32 below a row's largest.  The middles z + 8 s (rounded to bfloat16: they are small beside the
+//            numbers) and the sum of p are one more product, of rows of middles and of ones, with p as bfloat16.
 //            (About the zero points, with n for n - 8, the two parts nearly cancel over a long context: at 32000 keys the result was 5.2e-3
-//            off the one in 64 bits; it is 2.6e-3, of which bfloat16's last rounding alone makes 1.7e-3.)
+//            off the one in 64 bits; it is 2.3e-3, of which bfloat16's last rounding alone makes 1.7e-3.  p and p s each rounded to
+//            bfloat16: 2.7e-3, and 30.8 us instead of 31.8.)
 // The order of codes in a row (kv4.cuh) is the order in which these instructions' lanes want them: no shuffle, one 4 G-byte load of a
 // key row and one 2 G-byte load of a value row per lane.
 #include "kv4.cuh"
@@ -39,9 +41,9 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)_
 constexpr int kTile = 32;               // keys of a warp's step
 // Six warps a block and two blocks an SM leave a thread 168 registers, which the two chains of the loop need (eight warps with 128:
 // 8 x 8192 keys at 32 / 8 heads of 128 in 33.5 us instead of 29.8; blocks of four, three an SM: 30.2 us, and 37 uneven contexts of 600
-// keys 17.4 us instead of 13.7).
+// keys 17.4 us instead of 13.7; all before p s was rounded only once).
 constexpr int kWarps = 6, kResident = 2;
-constexpr float kStep = 8.f;
+constexpr float kStep = 8.f, kLift = 7.f;       // (log2 units) a reference's lag at most; p's factor
 constexpr int kHeads = 8;               // query heads of a block (columns of the products)
 template <int G> __host__ __device__ constexpr int stages() { return G == 4 ? 3 : 4; }
 template <int G> __host__ __device__ constexpr int stage_bytes() { return kTile * kKv4TokenBytes * G; }
@@ -74,10 +76,11 @@ __device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t times2(uint32_t x, uint32_t y) {           // two bfloat16 products
-    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
-    return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
+__device__ __forceinline__ float2 halves_of(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -327,13 +330,13 @@ attn_kv4_single_kernel(const SingleArgs a) {
         };
         relative();
         const float over = fmaxf(max3(max3(t[0][0], t[0][1], t[0][2]), t[0][3], t[1][0]), max3(t[1][1], t[1][2], t[1][3]));
-        if (__any_sync(0xffffffffu, !has[0] || !has[1] || over > kStep)) {
+        if (__any_sync(0xffffffffu, !has[0] || !has[1] || over > kStep + kLift)) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float top = fmaxf(fmaxf(sc[0][e], sc[0][2 + e]), fmaxf(sc[1][e], sc[1][2 + e])) * slh[e];
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                const float now = has[e] ? fmaxf(m[e], top) : top;
+                const float now = (has[e] ? fmaxf(m[e] + kLift, top) : top) - kLift;
                 const float f = has[e] ? ex2(m[e] - now) : 0.f;          // (the sums are 0, or NaN, before the first reference)
                 has[e] = now > -INFINITY;                                // (no key yet, or keys of NaN: any reference will do)
                 m[e] = has[e] ? now : 0.f;
@@ -347,7 +350,9 @@ attn_kv4_single_kernel(const SingleArgs a) {
     auto values = [&](const unsigned char* base, const float (&t)[2][4]) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const uint32_t p0 = transposed8x8(pack_pair(ex2(t[u][0]), ex2(t[u][1]))), p1 = transposed8x8(pack_pair(ex2(t[u][2]), ex2(t[u][3])));
+            const float2 f0 = halves_of(transposed8x8(half_pair(ex2(t[u][0]), ex2(t[u][1]))));
+            const float2 f1 = halves_of(transposed8x8(half_pair(ex2(t[u][2]), ex2(t[u][3]))));
+            const uint32_t p0 = pack_pair(f0.x, f0.y), p1 = pack_pair(f1.x, f1.y);
             const unsigned char* vu = base + 16 * u * 16 * G;
             const unsigned char* pu = base + 16 * u * 4 * G;
             {   // rows of the groups' middles, and a row of ones, over the 16 tokens, times p
@@ -361,7 +366,8 @@ attn_kv4_single_kernel(const SingleArgs a) {
             const Halves<G> vc = lds<Halves<G>>(vu + value_at + 8 * 16 * G), vd = lds<Halves<G>>(vu + value_at + 12 * 16 * G);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const uint32_t b0 = times2(p0, __byte_perm(wa.w[g], wb.w[g], 0x5410)), b1 = times2(p1, __byte_perm(wc.w[g], wd.w[g], 0x5410));
+                const uint32_t b0 = pack_pair(f0.x * kv4_step(wa.w[g]), f0.y * kv4_step(wb.w[g]));
+                const uint32_t b1 = pack_pair(f1.x * kv4_step(wc.w[g]), f1.y * kv4_step(wd.w[g]));
                 const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
                 const uint32_t ab = __byte_perm(va.w[g / 2], vb.w[g / 2], sel), cd = __byte_perm(vc.w[g / 2], vd.w[g / 2], sel);
                 mma16816(o[g][0], codes(ab), codes(ab >> 4), codes(cd), codes(cd >> 4), b0, b1);
