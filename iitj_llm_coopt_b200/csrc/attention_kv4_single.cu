@@ -450,11 +450,10 @@ attn_kv4_single_join_kernel(const SingleArgs a) {
     pdl_trigger();
     constexpr int N = D / 32;
     const int head = blockIdx.x * 4 + (threadIdx.x >> 5), item = blockIdx.y, lane = threadIdx.x & 31;
-    if (head >= a.heads) return;
     const int tok = a.items[item];
     const Span span = span_of(a, a.positions[tok]);
-    if (span.splits == 1) return;                        // one block wrote the result itself
-    pdl_wait();
+    pdl_wait();                                          // (before any way out: this grid must not end before the one it follows)
+    if (head >= a.heads || span.splits == 1) return;     // (one block wrote the result itself)
     const size_t at = ((size_t)item * a.heads + head) * a.max_splits;
     float top = -INFINITY;
     for (int s = lane; s < span.splits; s += 32) top = fmaxf(top, a.part_ml[2 * (at + s)]);
