@@ -50,7 +50,7 @@ _SIGNATURES = {
                            _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p],
     "llm_kv4_read": [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p],
     "llm_attention_kv4_general": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
-                                  _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p],
+                                  _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_void_p, _c_void_p],
     "llm_attention_kv4_single_supported": [_c_int, _c_int, _c_int, _c_int],
     "llm_attention_kv4_single_tile": [],
     "llm_attention_kv4_single_warps": [],
@@ -953,8 +953,18 @@ class Kernels:
                 self._kv4_single(q, table, request, positions, plan, out, shape, int(window), scale)
                 n_rows = 0
         if n_rows:
+            # few rows: their keys split over blocks, from 128 keys (a chunk for each of a block's warps) up
+            longest = max(max(meta.seq_lens_host), plan.context_bound or 0) if plan is not None else block_table.shape[1] * page_size
+            if window > 0:
+                longest = min(longest, int(window))
+            blocks = n_rows * kv_heads * -(-(heads // kv_heads) // 4)
+            splits = max(1, min(4 * self.sm_count // blocks, -(-longest // 128)))
+            part = None
+            if splits > 1:      # (allocated for the call, as in _kv4_single)
+                part = torch.empty(n_rows * heads * splits * (head_dim + 2), dtype=torch.float32, device=q.device)
+                self.launches += 1
             self._call("llm_attention_kv4_general", q_at, width, *table, _ptr(rows), n_rows, request.data_ptr(), positions.data_ptr(), out_at,
-                       out.shape[1], DTYPE_CODE[q.dtype], *shape, int(window), scale, self._stream())
+                       out.shape[1], DTYPE_CODE[q.dtype], *shape, int(window), scale, splits, _ptr(part), self._stream())
         return out
 
     def _kv4_prompt(self, q, table, plan, out, shape, window, scale):

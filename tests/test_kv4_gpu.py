@@ -417,3 +417,33 @@ def test_refusals(K):
                             z(0, 256), 4, 2, 64)
     assert empty.shape == (0, 256)
     assert K.rope_store_kv4(z(0, 512), None, None, None, 4, 2, 64, 0).shape == (0, 512)
+
+
+def test_a_captured_step_follows_its_contexts(K):
+    """One graph, replayed as the contexts grow from a few keys past several splits, each kernel behind the other: the single tokens
+    of both types and the general kernel (head size 96), with an early reader of the result behind each."""
+    for dtype, heads, kv, D in ((torch.bfloat16, 4, 1, 128), (torch.float32, 4, 1, 128), (torch.bfloat16, 4, 2, 96)):
+        lens = [1500, 1400]
+        q, cache, table, meta = case(14, lens, [1, 1], heads, kv, D, 16, dtype)
+        from iitj_llm_coopt_b200.kernels import attention_plan
+        meta.seq_lens_host = [1500, 1400]
+        attention_plan(meta, torch.device("cuda", 0)).context_bound = 1536
+        dq, dcache, out, ones = q.cuda(), cache.cuda(), torch.zeros(2, heads * D, dtype=dtype, device="cuda"), torch.ones(heads * D, device="cuda")
+        normed = torch.zeros_like(out)
+        K.attention_kv4(dq, dcache, meta, out, heads, kv, D)
+        K.rmsnorm_rows(out, ones, 1e-5, normed)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(3):
+                K.attention_kv4(dq, dcache, meta, out, heads, kv, D)
+                K.rmsnorm_rows(out, ones, 1e-5, normed)
+        for at in ([0, 3], [40, 1399], [700, 64], [1499, 1399]):
+            meta.positions.copy_(torch.tensor(at, dtype=torch.int32))
+            out.fill_(7.0)
+            graph.replay()
+            want, tol = P.attend(q[:, :heads * D], cache, table, [a + 1 for a in at], [1, 1], heads, kv, 16, D,
+                                 unit=P.U16 if dtype == torch.bfloat16 else P.U32)
+            assert bool(((out.cpu().double() - want).abs() <= tol).all()), at
+            again = torch.empty_like(out)
+            K.rmsnorm_rows(out, ones, 1e-5, again)
+            assert torch.equal(again, normed), at

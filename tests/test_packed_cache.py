@@ -114,7 +114,9 @@ def test_c_entry_points_refuse_before_they_touch_the_device():
         rc, text = store(**bad)
         assert rc == -1 and "rope_store_kv4" in text, bad
     assert call("llm_kv4_read", at, at, at, 0, 3, 2, 40, 16, None)[0] == -1
-    assert call("llm_attention_kv4_general", at, 256, at, at, 4, None, 3, at, at, at, 256, 1, 5, 2, 64, 16, 0, 0.1, None)[0] == -1     # 5 heads over 2
+    assert call("llm_attention_kv4_general", at, 256, at, at, 4, None, 3, at, at, at, 256, 1, 5, 2, 64, 16, 0, 0.1, 1, None, None)[0] == -1     # 5 heads over 2
+    for splits in (0, -1, 2):                           # none, and two without a place for their sums
+        assert call("llm_attention_kv4_general", at, 256, at, at, 4, None, 3, at, at, at, 256, 1, 4, 2, 64, 16, 0, 0.1, splits, None, None)[0] == -1
     assert call("llm_attention_kv4_single", at, 256, at, at, 4, at, 3, at, at, None, None, at, 256, 4, 2, 96, 16, 0, 0.1, 6, 1, None)[0] == -1
     assert call("llm_attention_kv4_single", at, 256, at, at, 4, at, 3, at, at, None, None, at, 256, 4, 2, 64, 12, 0, 0.1, 6, 1, None)[0] == -1
     assert call("llm_attention_kv4_single", at, 256, at, at, 4, at, 3, at, at, None, None, at, 256, 4, 2, 64, 16, 0, 0.1, 6, 2, None)[0] == -1     # no scratch
