@@ -10,9 +10,9 @@
 // and at the end the warps' sums are joined.  Keys outside [lo, pos] are not read.
 //
 // What bounds it is latency, of about 1700 instructions and the value rows' loads a chunk and warp; so the keys of few rows are split
-// over blocks, whose sums a second kernel joins.  Single tokens in float32: five contexts of 300 to 900 keys, 32 / 8 heads of 64, 24.0 us
-// (blocks of sixteen warps without splits: 40.6); one of 32000 keys, 32 / 8 heads of 128, 91 us; eight of 8192 128 us.  (Codes made
-// numbers by their place in 2^23 + n and values asked for eight at a time: 102 and 147 us.)
+// over blocks, whose sums a second kernel joins.  Single tokens in float32: five contexts of 300 to 900 keys, 32 / 8 heads of 64, 18.4 us
+// (without splits, by blocks of sixteen warps: 40.6; with half the lanes idle over heads of 64 numbers: 24.0); one of 32000 keys, 32 / 8
+// heads of 128, 81 us; eight of 8192 113 us.
 #include "kv4.cuh"
 
 namespace {
@@ -57,14 +57,15 @@ attn_kv4_general_kernel(const T* __restrict__ q, int q_stride, const uint8_t* __
         sq[h][c] = h < nh ? to_f32(q[(size_t)t * q_stride + (size_t)(h0 + h) * D + c]) * sl : 0.f;       // (scores in log2 units)
     }
     __syncthreads();
-    // this lane's value numbers: half-words lane and lane + 32 of a row
-    const int units = 8 * G;
-    float o[2][kGenHeads][4], m[kGenHeads], l[kGenHeads];
+    // this lane's value numbers: half-words lane and lane + 32 of a row; of 64 numbers, half-word lane % 16 of every other row
+    constexpr int kRows = GT == 2 ? 2 : 1, kUnits = GT ? 1 : 2;
+    const int units = 8 * G, unit = lane & (32 / kRows - 1);
+    float o[kUnits][kGenHeads][4], m[kGenHeads], l[kGenHeads];
 #pragma unroll
     for (int h = 0; h < kGenHeads; ++h) {
         m[h] = -INFINITY; l[h] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[0][h][e] = o[1][h][e] = 0.f;
+        for (int r = 0; r < kUnits; ++r) o[r][h][0] = o[r][h][1] = o[r][h][2] = o[r][h][3] = 0.f;
     }
     for (int k0 = first + warp * 32; k0 <= last; k0 += kGenWarps * 32) {
         const int n = min(32, last + 1 - k0), key = k0 + min(lane, n - 1);
@@ -111,31 +112,38 @@ attn_kv4_general_kernel(const T* __restrict__ q, int q_stride, const uint8_t* __
             m[h] = top;
             l[h] = l[h] * f + p;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { o[0][h][e] *= f; o[1][h][e] *= f; }
+            for (int r = 0; r < kUnits; ++r) { o[r][h][0] *= f; o[r][h][1] *= f; o[r][h][2] *= f; o[r][h][3] *= f; }
             sp[warp][h][lane] = p;
         }
         __syncwarp();
 #pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-            const int voff = __shfl_sync(0xffffffffu, off, i);
-            const uint8_t* vb = cache + ((size_t)__shfl_sync(0xffffffffu, page, i) * kv_heads + hk) * block_bytes;
+        for (int i = 0; i < n; i += kRows) {
+            const int at = i + (kRows > 1 ? lane / 16 : 0), row = min(at, n - 1);        // (behind the last key: it again, times 0)
+            const int voff = __shfl_sync(0xffffffffu, off, row);
+            const uint8_t* vb = cache + ((size_t)__shfl_sync(0xffffffffu, page, row) * kv_heads + hk) * block_bytes;
             const uint16_t* vc = reinterpret_cast<const uint16_t*>(vb + kv4_value_codes(page_size, G) + (size_t)voff * 16 * G);
             const uint32_t* vpar = reinterpret_cast<const uint32_t*>(vb + kv4_value_par(page_size, G) + (size_t)voff * 4 * G);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int u = lane + 32 * r;
-                if (u < units) {
+            for (int r = 0; r < kUnits; ++r) {
+                const int u = unit + 32 * r;
+                if (GT || u < units) {
                     const uint32_t w = vc[u], p4 = vpar[u % G];
                     const float step = kv4_step(p4), zero = kv4_zero(p4);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float x = fmaf(step, (float)((w >> (4 * e)) & 15u), zero);
 #pragma unroll
-                        for (int h = 0; h < kGenHeads; ++h) o[r][h][e] = fmaf(sp[warp][h][i], x, o[r][h][e]);
+                        for (int h = 0; h < kGenHeads; ++h) o[r][h][e] = fmaf(sp[warp][h][at], x, o[r][h][e]);
                     }
                 }
             }
         }
+    }
+    if constexpr (kRows > 1) {
+#pragma unroll
+        for (int h = 0; h < kGenHeads; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[0][h][e] += __shfl_xor_sync(0xffffffffu, o[0][h][e], 16);
     }
     auto top_of = [&](int h) {
         float top = sm[0][h];
@@ -155,7 +163,7 @@ attn_kv4_general_kernel(const T* __restrict__ q, int q_stride, const uint8_t* __
                 const float top = top_of(h);
                 const float f = gen_weight(sm[w][h], sl_sum[w][h], top);
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
+                for (int r = 0; r < kUnits; ++r) {
                     const int u = lane + 32 * r;
                     if (u < units) {
                         const int c = u / G, g = u - c * G, at = 32 * g + 8 * (c >> 1) + (c & 1);
