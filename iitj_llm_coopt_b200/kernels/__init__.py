@@ -744,7 +744,7 @@ class Kernels:
         """`rope_store` into a packed cache: rotates the queries, rotates and packs the keys, packs the values and stores both in
         every token's cache slot (a slot below 0: nowhere).
 
-        cache_layer: uint8 [pages, bytes] (csrc/kv4.cuh); slots may be None (rotate only).  tables: (cos, sin) of `rope_tables`
+        cache_layer: uint8 [pages, bytes] (csrc/kv4.cuh); slots may be None (rotate only); no slot twice.  tables: (cos, sin) of `rope_tables`
         (None with rotary_dim 0).  `qkv` may be a PartialSums of up to eight parts: they are added on the way.  `q_out`
         [tokens, heads * head_dim] receives the queries; without it they are rotated in place in qkv, whose keys and values stay as
         they are.  Returns the tensor that holds the rotated queries."""
