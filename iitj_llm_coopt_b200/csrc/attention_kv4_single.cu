@@ -26,6 +26,11 @@
 //            (About the zero points, with n for n - 8, the two parts nearly cancel over a long context: at 32000 keys the result was 5.2e-3
 //            off the one in 64 bits; it is 2.3e-3, of which bfloat16's last rounding alone makes 1.7e-3.  p and p s each rounded to
 //            bfloat16: 2.7e-3, and 30.8 us instead of 31.8.)
+//   range    p is up to 2^15 here, so p s would leave float32 and bfloat16 from steps of 2^113 on, and so would the products' 2^17 times a
+//            key's step.  From the first tile with a value's step or zero point of 2^65 or more a warp's sums are taken times 2^-64
+//            (its reference counts that); a tile with such a key has its stored words multiplied by 2^-64 where they lie in shared memory
+//            and its scores made again, with a scale times 2^64.  The vote on the reference
+//            finds out; looking at the words costs 3% (8 requests over 8192: 31.5 to 32.5 us).
 // The order of codes in a row (kv4.cuh) is the order in which these instructions' lanes want them: no shuffle, one 4 G-byte load of a
 // key row and one 2 G-byte load of a value row per lane.
 #include "kv4.cuh"
@@ -114,6 +119,16 @@ __device__ __forceinline__ uint32_t middles(uint32_t a, uint32_t b) {
 }
 
 template <int G> struct alignas(4 * G) Words { uint32_t w[G]; };
+
+// (s, z) words of a token in which a number is 2^65 or more in size (both top bits of its exponent are set), or NaN.
+template <int G> __device__ __forceinline__ uint32_t loud(const Words<G>& x) {
+    uint32_t both = 0u;
+#pragma unroll
+    for (int g = 0; g < G; ++g) both |= x.w[g] & (x.w[g] << 1);
+    return both & 0x40004000u;
+}
+constexpr float kQuiet = 5.42101086242752217e-20f, kLoud = 18446744073709551616.f;      // 2^-64 and 2^64
+constexpr float kLoudLog = 64.f;
 template <int G> struct alignas(2 * G) Halves { uint32_t w[G / 2]; };      // G half-words of a value row
 template <typename W> __device__ __forceinline__ W lds(const unsigned char* at) { return *reinterpret_cast<const W*>(at); }
 
@@ -269,6 +284,7 @@ attn_kv4_single_kernel(const SingleArgs a) {
         }
     }
     float o[G][2][4], oz[4] = {0.f, 0.f, 0.f, 0.f}, m[2] = {0.f, 0.f};
+    float quiet = 1.f;               // 2^-64 once a value of this warp was loud: in all its sums
     bool has[2] = {false, false};    // m holds a reference (in log2 units)
 #pragma unroll
     for (int g = 0; g < G; ++g)
@@ -282,6 +298,9 @@ attn_kv4_single_kernel(const SingleArgs a) {
     const int kz_at = kKeyPar + par_at + 4 * (G == 4 ? j : j & 1), vz_at = kValuePar + j * 4 * G + 4 * (r8 < G ? r8 : 0);
     const uint32_t z_keep = r8 < G ? 0xffffffffu : 0u, z_add = r8 == G ? 0x3f803f80u : 0u;         // rows of oz: z of the groups, then 1
 
+    // Whether token x of a tile (lane x) has loud numbers in its key or its value.
+    auto loud_key = [&](const unsigned char* base) { return loud<G>(lds<Words<G>>(base + kKeyPar + lane * 4 * G)); };
+    auto loud_value = [&](const unsigned char* base) { return loud<G>(lds<Words<G>>(base + kValuePar + lane * 4 * G)); };
     auto scores = [&](const unsigned char* base, float (&sc)[2][4]) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -311,29 +330,54 @@ attn_kv4_single_kernel(const SingleArgs a) {
     };
     // Exponents t of a tile relative to the reference m.  It follows the maximum in steps of 2^8 only (p stays below 2^8), so that in
     // most tiles one vote is all there is to do; a head without a reference yet takes the tile's maximum.
-    auto exponents = [&](int i, float (&sc)[2][4], float (&t)[2][4]) {
+    auto exponents = [&](int i, unsigned char* base, uint32_t odd, float (&sc)[2][4], float (&t)[2][4]) {
         const int key0 = (first + i * stride) * kTile;
-        if (key0 + kTile - 1 > pos || key0 < lo) {
+        float sl[2] = {slh[0], slh[1]};
+        auto mask = [&] {
+            if (key0 + kTile - 1 > pos || key0 < lo) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int key = key0 + 16 * u + 8 * e + trow;
-                    if (key > pos || key < lo) sc[u][2 * e] = sc[u][2 * e + 1] = -INFINITY;
-                }
-        }
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = key0 + 16 * u + 8 * e + trow;
+                        if (key > pos || key < lo) sc[u][2 * e] = sc[u][2 * e + 1] = -INFINITY;
+                    }
+            }
+        };
         auto relative = [&] {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) t[u][e] = fmaf(sc[u][e], slh[e & 1], -m[e & 1]);
+                for (int e = 0; e < 4; ++e) t[u][e] = fmaf(sc[u][e], sl[e & 1], -m[e & 1]);
         };
+        mask();
         relative();
         const float over = fmaxf(max3(max3(t[0][0], t[0][1], t[0][2]), t[0][3], t[1][0]), max3(t[1][1], t[1][2], t[1][3]));
-        if (__any_sync(0xffffffffu, !has[0] || !has[1] || over > kStep + kLift)) {
+        if (__any_sync(0xffffffffu, !has[0] || !has[1] || over > kStep + kLift || odd != 0u)) {
+            if (__any_sync(0xffffffffu, odd != 0u)) {
+                if (__any_sync(0xffffffffu, loud_key(base) != 0u)) {     // the scores once more, over words times 2^-64
+                    Words<G>* key = reinterpret_cast<Words<G>*>(base + kKeyPar + lane * 4 * G);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) key->w[g] = pack_pair(kv4_step(key->w[g]) * kQuiet, kv4_zero(key->w[g]) * kQuiet);
+                    __syncwarp();
+                    scores(base, sc);
+                    mask();
+                    sl[0] *= kLoud;
+                    sl[1] *= kLoud;
+                }
+                if (quiet == 1.f && __any_sync(0xffffffffu, loud_value(base) != 0u)) {
+                    quiet = kQuiet;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        oz[e] *= kQuiet;
+#pragma unroll
+                        for (int g = 0; g < G; ++g) { o[g][0][e] *= kQuiet; o[g][1][e] *= kQuiet; }
+                    }
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float top = fmaxf(fmaxf(sc[0][e], sc[0][2 + e]), fmaxf(sc[1][e], sc[1][2 + e])) * slh[e];
+                float top = fmaxf(fmaxf(sc[0][e], sc[0][2 + e]), fmaxf(sc[1][e], sc[1][2 + e])) * sl[e];
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                 const float now = (has[e] ? fmaxf(m[e] + kLift, top) : top) - kLift;
@@ -350,8 +394,9 @@ attn_kv4_single_kernel(const SingleArgs a) {
     auto values = [&](const unsigned char* base, const float (&t)[2][4]) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const float2 f0 = halves_of(transposed8x8(half_pair(ex2(t[u][0]), ex2(t[u][1]))));
-            const float2 f1 = halves_of(transposed8x8(half_pair(ex2(t[u][2]), ex2(t[u][3]))));
+            float2 f0 = halves_of(transposed8x8(half_pair(ex2(t[u][0]), ex2(t[u][1]))));
+            float2 f1 = halves_of(transposed8x8(half_pair(ex2(t[u][2]), ex2(t[u][3]))));
+            f0.x *= quiet; f0.y *= quiet; f1.x *= quiet; f1.y *= quiet;
             const uint32_t p0 = pack_pair(f0.x, f0.y), p1 = pack_pair(f1.x, f1.y);
             const unsigned char* vu = base + 16 * u * 16 * G;
             const unsigned char* pu = base + 16 * u * 4 * G;
@@ -381,19 +426,20 @@ attn_kv4_single_kernel(const SingleArgs a) {
         float sc[2][4], t[2][4];
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
         __syncwarp();                                    // every lane's copies of the tile are there
-        const unsigned char* base = ring;
+        unsigned char* base = ring;
         scores(base, sc);
-        exponents(0, sc, t);
+        exponents(0, base, loud_key(base) | loud_value(base), sc, t);
         for (int i = 0; i + 1 < n_tiles; ++i) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
             __syncwarp();
-            const unsigned char* next = ring + ((i + 1) % kStages) * kStageBytes;
+            unsigned char* next = ring + ((i + 1) % kStages) * kStageBytes;
             scores(next, sc);
             values(base, t);
+            const uint32_t odd = loud_key(next) | loud_value(next);
             __syncwarp();                                // every lane has what it wants of tile i's stage
             load_tile(i + kStages, page_next);
             page_next = fetch_page(i + kStages + 1);
-            exponents(i + 1, sc, t);
+            exponents(i + 1, next, odd, sc, t);
             base = next;
         }
         values(base, t);
@@ -407,7 +453,7 @@ attn_kv4_single_kernel(const SingleArgs a) {
 #pragma unroll
         for (int g = 0; g < G; ++g) zg[g][e] = __shfl_sync(0xffffffffu, oz[e], 4 * g + j);
         l[e] = __shfl_sync(0xffffffffu, oz[e], 4 * G + j);
-        if (r8 == 0) { sm_m[warp][2 * j + e] = has[e] ? m[e] : -INFINITY; sm_l[warp][2 * j + e] = l[e]; }
+        if (r8 == 0) { sm_m[warp][2 * j + e] = has[e] ? (quiet == 1.f ? m[e] : m[e] + kLoudLog) : -INFINITY; sm_l[warp][2 * j + e] = l[e]; }
     }
     __syncthreads();                                     // every warp is done with its stages: they become the sums' place
     float* part = reinterpret_cast<float*>(smem);        // [kWarps][kHeads][D]
