@@ -7,15 +7,17 @@
 //   s = bfloat16((max x - z) * (1 / 15))   (0 below the smallest normal float32: the group is its zero point)
 //   n = clamp(rint((x - z) * (1 / s)), 0, 15)
 //
-// all in float32, rounded operation by operation, so the codes are defined to the bit.  A number is off by at most s / 2 and what
-// rounding s to bfloat16 adds at the top code (15 s 2^-9).  z and s are not finite if a number of the group is not (or if the group
-// spans more than float32 does); a token with such a group in its key or its value keeps, in that head, a key whose z and s are NaN
-// and a value of zeros: whoever sees the token gets NaN, and whoever does not see it cannot get one from a probability of 0 times it.
+// all in float32, rounded operation by operation, so the codes are defined to the bit.  A number is off by at most s / 2 (rounding s to
+// bfloat16 moves the top code's number by up to 15 s 2^-8, which is less) and float32's roundings.  z + 15 s is not finite if a number of
+// the group is not, if the group spans more than float32 does, or if it lies so near float32's largest number that a step rounded up
+// passes it; a token with such a group in its key or its value keeps, in that head, a key whose z and s are NaN and a value of zeros:
+// whoever sees the token gets NaN, and whoever does not see it cannot get one from a probability of 0 times it.  Every value that the
+// cache holds is finite.
 //
 // A page is kv_heads blocks, one per key/value head; a block is
 //   [page_size][16 G] key codes, [page_size][4 G] key (s, z), [page_size][16 G] value codes, [page_size][4 G] value (s, z)
-// 40 G bytes a token (160 at D = 128, where bfloat16 takes 512), and one block is one contiguous run of bytes: what a decode CTA
-// wants of a page is one bulk copy.  page_size is a multiple of 4, so every region starts on a 16-byte boundary.
+// 40 G bytes a token (160 at D = 128, where bfloat16 takes 512), and one block is one contiguous run of bytes.  page_size is a multiple
+// of 4, so every region starts on a 16-byte boundary and is read and copied in pieces of 16 bytes.
 // Which nibble is which number follows from the matrix instructions that read them without a shuffle (attention_kv4_single.cu):
 //   key row    word j G + g (32 bits, j < 4):       numbers 32 g + 8 j + {0, 2, 4, 6, 1, 3, 5, 7}, low nibble first
 //   value row  half-word c G + g (16 bits, c < 8):  numbers 32 g + 8 (c / 2) + (c % 2) + {0, 2, 4, 6}, low nibble first

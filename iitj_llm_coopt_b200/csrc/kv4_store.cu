@@ -86,7 +86,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // Packs 32 numbers held by 4 neighbouring lanes, eight each (all lanes of the warp call): the lane's code word, the group's (s, z), and
-// whether anything of the lane's, or s or z, is not finite.
+// whether anything of the lane's, or s or z, or the number of the top code, is not finite.  (s may be rounded up, by 2^-8 of it: float32
+// numbers next to the largest one would come back as infinity.)
 //
 // Four instructions a number, for this is where the kernel's instructions go: x - z, times r, plus 1.5 2^23 (whose last bit counts 1: the
 // sum's low bits are the product rounded to the nearest even), and a multiply-add that shifts those bits into the word; what the
@@ -106,7 +107,7 @@ __device__ __forceinline__ void pack_group(const Eight& v, uint32_t& word, uint3
     const float z = __bfloat162float(__float2bfloat16_rd(lo));
     float s = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, z), 1.0f / 15.0f)));
     if (s < 1.17549435e-38f) s = 0.f;
-    bad = zeros != 0.f || !finite(z) || !finite(s);
+    bad = zeros != 0.f || !finite(fmaf(15.f, s, z));     // (which z or s that is not finite makes NaN or infinite too)
     const float r = s > 0.f ? __frcp_rn(s) : 0.f;
     constexpr uint32_t kOnTop = 0x4b400000u;            // 1.5 2^23
     word = 0u;
