@@ -314,12 +314,13 @@ class CacheManager:
         full = [self.groups[gi].pool.num_pages for gi in self.paged if self.groups[gi].need.window <= 0]
         return min(full, default=self.num_pages) * self.page_size
 
-    def can_admit(self, tokens: int, watermark: float = 0.0) -> bool:
+    def can_admit(self, tokens: int, watermark: float = 0.0, forked: int = 0) -> bool:
         """True if a new request's first `tokens` tokens fit every paged group while `watermark` of the group's
-        pool stays free (the reference's admission rule, engine/engine.py:124-140, per group)."""
+        pool stays free (the reference's admission rule, engine/engine.py:124-140, per group).  `forked`: the tokens
+        that it takes over as a fork, whose full pages it shares."""
         for gi in self.paged:
             g = self.groups[gi]
-            if g.pages_for(tokens) > g.pool.num_free - int(watermark * g.pool.num_pages):
+            if g.pages_for(tokens) - forked // self.page_size > g.pool.num_free - int(watermark * g.pool.num_pages):
                 return False
         return True
 

@@ -62,8 +62,11 @@ class Engine:
         return self.add_request(seq)
 
     def new_sequences(self, n, prompt, max_tokens, temperature=0.0, ignore_eos=False, seed=None, on_output=None) -> list:
-        """`n` sequences of one prompt.  The first computes the prompt; the others fork from it as soon as that step is launched
-        (`_branch`), so the prompt is computed once and its full cache pages are held once.  A given seed is `seed + i` for sequence i."""
+        """`n` sequences of one prompt.  The first computes the prompt; the others wait until that step is launched and are then
+        admitted as any request is (first in the queue), but fork from one of the prompt's sequences that is in the cache, so the prompt
+        is computed once and its full cache pages are held once.  One that finds none to fork from (layers that keep state; a window
+        that has passed the prompt's end; all of them finished or preempted) computes the prompt itself.  A given seed is `seed + i`
+        for sequence i."""
         if n < 1:
             raise ValueError("n must be at least 1")
         first = self.new_sequence(prompt, max_tokens, temperature, ignore_eos, seed, on_output)
@@ -74,26 +77,17 @@ class Engine:
             self._next_id += 1
         if len(prompt) > 1:
             first.branches = list(rest)
+            family = [first] + rest
+            for s in family:
+                s.family = family
         else:
             self.scheduler.waiting.extend(rest)            # a prompt of one token: nothing to share
         return [first] + rest
 
     def _branch(self, seq) -> None:
-        """Forks the branches of a sequence whose prompt's last portion has been launched.  A branch starts with all of the prompt
-        but its last token in the cache and feeds that token itself, which gives it logits of its own to draw from.  Where the cache
-        cannot fork (no page or slot free, state that cannot be taken back by a token) the branch waits for admission and computes the
-        prompt itself."""
-        stored, waiting = seq.prompt_len - 1, []
-        sched = self.scheduler
-        for child in seq.branches:
-            if len(sched.running) + sched.held_slots < self.policy.max_num_seqs and self.cache.can_fork(seq.seq_id, stored):
-                self.runner.fork(seq.seq_id, child.seq_id, stored)
-                child.num_computed = stored
-                sched.running.append(child)
-            else:
-                waiting.append(child)
+        """Sends the branches of a sequence to the head of the queue: its prompt's last portion has been launched, or it ended before."""
+        self.scheduler.waiting.extendleft(reversed(seq.branches))
         seq.branches = []
-        sched.waiting.extendleft(reversed(waiting))
 
     def release(self, seq) -> None:
         if self.cache.has(seq.seq_id):
@@ -104,8 +98,7 @@ class Engine:
         seq.finish_time = time.perf_counter()
         if seq in self.scheduler.running:
             self.scheduler.running.remove(seq)
-        self.scheduler.waiting.extendleft(reversed(seq.branches))     # it ended before its prompt was computed
-        seq.branches = []
+        self._branch(seq)
         self.release(seq)
         key = "request_failure_total" if reason == "out_of_pages" else "request_success_total"
         self.counters[key] += 1
@@ -184,7 +177,7 @@ class Engine:
         for s, end in plan.chunks:
             self.counters["prompt_tokens_total"] += end - s.num_computed
             s.num_computed = end
-        for s in [s for s, _ in plan.chunks] + plan.decodes:
+        for s in reversed([s for s, _ in plan.chunks] + plan.decodes):
             if s.branches and self.cache.num_tokens(s.seq_id) >= s.prompt_len:
                 self._branch(s)
         return self._sample(logits, sampled, [s.num_generated for s in sampled], sum(len(e.tokens) for e in entries), t0)

@@ -8,7 +8,9 @@ Three phases per step, as the reference's Scheduler.schedule (engine/engine.py:9
   2. running prefills, oldest first, each cut to what is left of the step's token budget;
      a portion whose pages do not fit is skipped this step;
   3. admissions from the waiting queue while the budget, `max_num_seqs` and the page
-     watermark allow; the first request that does not fit stops admission.
+     watermark allow; the first request that does not fit stops admission.  A request whose prompt is in
+     the cache, as another sequence's of the same prompt, is admitted as a fork of that one: all of the
+     prompt but its last token is there, and it feeds that token (and what it had generated) itself.
 Token bookkeeping (engine/engine.py:8-11): `tokens` = prompt + generated, the cache holds the
 first `num_computed`; decoding is "one remaining token"; a preempted sequence is recomputed
 from position 0 as one (chunked) prefill of prompt + generated.
@@ -49,7 +51,8 @@ class Sequence:
     finished: bool = False
     finish_reason: str | None = None
     num_preemptions: int = 0
-    branches: list = field(default_factory=list)    # sequences of the same prompt that fork from this one once it is computed
+    branches: list = field(default_factory=list)    # sequences of the same prompt that wait for this one to compute it
+    family: list = field(default_factory=list, repr=False, compare=False)      # all sequences of that prompt, itself among them
     pending_row: int | None = None      # row of the step in flight whose sampled id is this sequence's last token
 
     def __post_init__(self):
@@ -90,6 +93,10 @@ class Scheduler:
         seq.num_preemptions += 1
         self.counters["num_preemptions_total"] = self.counters.get("num_preemptions_total", 0) + 1
         self.waiting.appendleft(seq)
+
+    def _fork_source(self, seq):
+        """A sequence of the same prompt that `seq` can be forked from, or None."""
+        return next((s for s in seq.family if s is not seq and self.cache.can_fork(s.seq_id, seq.prompt_len - 1)), None)
 
     def schedule(self) -> Plan:
         while True:
@@ -141,13 +148,19 @@ class Scheduler:
         while self.waiting and budget > 0 and len(self.running) + self.held_slots < pol.max_num_seqs:
             i = pol.pick_next(self.waiting, self.engine)
             s = self.waiting[i]
-            end = s.num_computed + min(s.remaining, budget)
+            source = self._fork_source(s)
+            stored = s.prompt_len - 1 if source is not None else 0
+            end = stored + min(len(s.tokens) - stored, budget)
             # (the watermark is waived while nothing runs, so that a prompt that fits the pool is admitted eventually)
-            if not cache.can_admit(end, pol.watermark if self.running else 0.0) or not pol.admit(s, self.engine):
+            if not cache.can_admit(end, pol.watermark if self.running else 0.0, stored) or not pol.admit(s, self.engine):
                 break
             del self.waiting[i]
             self.running.append(s)
-            cache.admit(s.seq_id)
+            if source is not None:
+                (self.engine.runner if self.engine is not None else cache).fork(source.seq_id, s.seq_id, stored)
+                s.num_computed = stored
+            else:
+                cache.admit(s.seq_id)
             cache.ensure(s.seq_id, end)
             if s.remaining == 1:
                 plan.decodes.append(s)
