@@ -433,15 +433,17 @@ class CacheManager:
     # ---- forks -----------------------------------------------------------------------------
     # A fork starts as a request whose first tokens are another's: it holds the same full pages (nobody writes in a full
     # page again), and of the page that both would go on writing a copy of its own.
+    @property
+    def forkable(self) -> bool:
+        """True if no layer keeps state (a state holds all tokens so far: it cannot be taken back to fewer)."""
+        return len(self.paged) == len(self.groups)
+
     def can_fork(self, parent, tokens: int) -> bool:
         """True if `fork` can give a new request the parent's first `tokens` tokens: they are stored and their pages still
-        there, a request slot and, where the tokens end inside a page, a page per group are free, and no layer keeps state (a
-        state holds all tokens so far: it cannot be taken back to fewer)."""
-        if not self.free_slots or not 0 < tokens <= self.stored.get(parent, 0):
+        there, a request slot and, where the tokens end inside a page, a page per group are free, and no layer keeps state."""
+        if not self.forkable or not self.free_slots or not 0 < tokens <= self.stored.get(parent, 0):
             return False
         for g in self.groups:
-            if not isinstance(g, PagedGroup):
-                return False
             table = g.tables[parent]
             if any(p < 0 for p in table[g.first_needed_page(tokens):g.pages_for(tokens)]):
                 return False

@@ -11,6 +11,9 @@ Three phases per step, as the reference's Scheduler.schedule (engine/engine.py:9
      watermark allow; the first request that does not fit stops admission.  A request whose prompt is in
      the cache, as another sequence's of the same prompt, is admitted as a fork of that one: all of the
      prompt but its last token is there, and it feeds that token (and what it had generated) itself.
+     While such a sequence is still computing the prompt, the request waits; and the slots that the
+     waiting sequences of a running one's prompt will take are not given to requests behind them, which
+     would keep them out until nobody holds the prompt any more.
 Token bookkeeping (engine/engine.py:8-11): `tokens` = prompt + generated, the cache holds the
 first `num_computed`; decoding is "one remaining token"; a preempted sequence is recomputed
 from position 0 as one (chunked) prefill of prompt + generated.
@@ -98,6 +101,12 @@ class Scheduler:
         """A sequence of the same prompt that `seq` can be forked from, or None."""
         return next((s for s in seq.family if s is not seq and self.cache.can_fork(s.seq_id, seq.prompt_len - 1)), None)
 
+    def _prompt_under_way(self, seq) -> bool:
+        """True if a sequence in the cache is computing the prompt that `seq` could then be forked from."""
+        cache = self.cache
+        return cache.forkable and any(s is not seq and cache.has(s.seq_id) and cache.num_tokens(s.seq_id) < seq.prompt_len - 1
+                                      for s in seq.family)
+
     def schedule(self) -> Plan:
         while True:
             plan = self._schedule_once()
@@ -145,10 +154,13 @@ class Scheduler:
                 budget -= end - s.num_computed
 
         # 3. admissions
-        while self.waiting and budget > 0 and len(self.running) + self.held_slots < pol.max_num_seqs:
+        promised = sum(len(s.branches) for s in self.running)
+        while self.waiting and budget > 0 and len(self.running) + self.held_slots + promised < pol.max_num_seqs:
             i = pol.pick_next(self.waiting, self.engine)
             s = self.waiting[i]
             source = self._fork_source(s)
+            if source is None and self._prompt_under_way(s):
+                break
             stored = s.prompt_len - 1 if source is not None else 0
             end = stored + min(len(s.tokens) - stored, budget)
             # (the watermark is waived while nothing runs, so that a prompt that fits the pool is admitted eventually)
@@ -156,6 +168,7 @@ class Scheduler:
                 break
             del self.waiting[i]
             self.running.append(s)
+            promised += len(s.branches)
             if source is not None:
                 (self.engine.runner if self.engine is not None else cache).fork(source.seq_id, s.seq_id, stored)
                 s.num_computed = stored

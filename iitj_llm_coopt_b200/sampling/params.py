@@ -5,7 +5,8 @@ The reference's per-request knobs are `max_tokens`, `temperature` (0 = greedy) a
 (engine/spec_decode.py:12-17).  `seed` is added so that a request's random draws can be
 fixed independently of the engine's seed and of what else is running.  `n` asks for several
 completions of one prompt: the prompt is computed once and its cache pages are shared
-(cache/manager.py, fork); completion i draws with seed + i if a seed is given.
+(cache/manager.py, fork; Engine.new_sequences says when one has to compute it again);
+completion i draws with seed + i if a seed is given.
 """
 from __future__ import annotations
 
