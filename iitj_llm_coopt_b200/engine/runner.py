@@ -324,7 +324,10 @@ class ModelRunner:
             cols = min(widths[g], matrix.shape[1])
             tab[:, :cols] = matrix[slot_rows, :cols]
             tab[:, cols:] = 0
-            put(f"slots{g}", tab[token_request, page_of].astype(np.int64) * ps + offset_in)
+            cells = tab[token_request, page_of].astype(np.int64) * ps + offset_in
+            if pad and cache.groups[g].need.bits:
+                cells[T - pad:] = -1       # a packed store wants every slot once: padding rows leave the padding page as it is
+            put(f"slots{g}", cells)
         self._meta[:off].copy_(self._pinned[:off], non_blocking=True)
         self.copied_bytes = 4 * off            # what this step sent to the device (benchmarks report it)
         if self._meta.is_cuda:
