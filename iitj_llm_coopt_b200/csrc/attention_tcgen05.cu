@@ -35,6 +35,8 @@
 //   values   over such a power 2^e as well.  P of the tile is taken times 2^e, so O needs nothing; l takes it back.  The reference
 //            M follows the scores plus e: what float16 flushes lies 2^-29 below the tile's largest value, or 2^-32 below the row's
 //            largest product
+// A power holds the tokens of a tile down to 2^-22 of the largest.  Where one lies below that (or keys below 2^-89, values below 2^-49), a
+// query that sees it and not the loud one would lose it; the CTA then works its rows out one by one in float32 (attend_row).
 // Measured, 32 heads over 8 of 128 numbers: a prompt of 2048 tokens 62.7 us (over a bfloat16 cache 47), of 8192 tokens 651 us, 845
 // TFLOP/s (492 to 530).  Unpacking does not bound it: with the codes left as they are it took as long.  What it has more than the other form
 // is the maximum before the probabilities, the exponents, and registers: 14 warps leave a thread 128.
@@ -240,6 +242,9 @@ __device__ __forceinline__ uint32_t top_values(uint32_t word) { return word >> 8
 __device__ __forceinline__ float top_down(uint32_t e8) { return __uint_as_float((268u - e8) << 23); }
 __device__ __forceinline__ float top_up(uint32_t e8) { return __uint_as_float((e8 - 14u) << 23); }
 constexpr uint32_t kKeyLeast = 60u, kValueLeast = 100u;      // numbers all below 2^-67 or 2^-27 are taken as if one were that large
+// A tile's tokens may lie this many powers of two below its largest: float16 then holds their numbers within 2^-17 of the token's own
+// largest.  A tile with a token further down (and not 0) is beyond the products: a query that sees that one alone would lose it.
+constexpr uint32_t kReach = 22u;
 
 struct AttnArgs {
     const int* block_table;
@@ -255,8 +260,83 @@ struct AttnArgs {
     int pairs;                    // CTAs per key/value group: ceil(heads per group / per_cta)
     float sl;                     // softmax scale * log2(e)
     const uint8_t* packed;        // the packed cache layer
+    const bf16* q;                // the queries, for rows that are worked on one by one
+    int q_stride;
     int one_pass;                 // tiles after a request's first: one softmax pass (see the kernel); 0: always two (IITJ_ATTN_ONE_PASS=0)
 };
+
+// One query row and head over the keys first .. last of a packed cache, by one thread in float32: what the kernel below does where a tile's
+// tokens are too far apart in size for float16 (kReach).  As slow as it is rare: 64 numbers at a time, every score made anew for them (a prompt of 2048 tokens with one value of 2^26
+// takes 13.3 ms where it takes 63 us without, 32 heads over 8 of 128).
+// part: where the sums go, relative to the reference that is stored beside them, or null: `out` takes the result.
+template <int D>
+__device__ __noinline__ void attend_row(const AttnArgs& a, int tok, int head, int hk, int req, int first, int last, float* part, float* part_ml) {
+    constexpr int G = D / 32;
+    const int ps = a.page_size;
+    const int* table = a.block_table + (size_t)req * a.table_width;
+    const size_t block_bytes = kv4_block_bytes(ps, G);
+    const bf16* q = a.q + (size_t)tok * a.q_stride + (size_t)head * D;
+#pragma unroll 1
+    for (int half = 0; half < G / 2; ++half) {
+        float o[64], m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) o[i] = 0.f;
+#pragma unroll 1
+        for (int key = first; key <= last; ++key) {
+            const int lp = key / ps, off = key - lp * ps;
+            const uint8_t* block = a.packed + ((size_t)table[lp] * a.kv_heads + hk) * block_bytes;
+            const uint32_t* codes = reinterpret_cast<const uint32_t*>(block + (size_t)off * 16 * G);
+            const uint32_t* par = reinterpret_cast<const uint32_t*>(block + kv4_key_par(ps, G) + (size_t)off * 4 * G);
+            float s = 0.f;
+#pragma unroll 1
+            for (int g = 0; g < G; ++g) {
+                const float step = kv4_step(par[g]), zero = kv4_zero(par[g]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w = codes[j * G + g];
+                    const uint4 r = *reinterpret_cast<const uint4*>(q + 32 * g + 8 * j);
+                    const uint32_t qw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s = fmaf(__uint_as_float(qw[e] << 16), fmaf(step, (float)(w >> kv4_bit(2 * e) & 15u), zero), s);
+                        s = fmaf(__uint_as_float(qw[e] & 0xffff0000u), fmaf(step, (float)(w >> kv4_bit(2 * e + 1) & 15u), zero), s);
+                    }
+                }
+            }
+            s *= a.sl;
+            const float top = fmaxf(m, s), mu = top == -INFINITY ? 0.f : top;
+            const float f = exp2f(m - mu), p = exp2f(s - mu);
+            m = top;
+            l = l * f + p;
+            const uint16_t* vc = reinterpret_cast<const uint16_t*>(block + kv4_value_codes(ps, G) + (size_t)off * 16 * G);
+            const uint32_t* vpar = reinterpret_cast<const uint32_t*>(block + kv4_value_par(ps, G) + (size_t)off * 4 * G);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const uint32_t pw = vpar[2 * half + g];
+                const float step = kv4_step(pw), zero = kv4_zero(pw);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const uint32_t w = vc[c * G + 2 * half + g];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float& to = o[32 * g + 8 * (c >> 1) + (c & 1) + 2 * e];
+                        to = fmaf(p, fmaf(step, (float)(w >> (4 * e) & 15u), zero), to * f);
+                    }
+                }
+            }
+        }
+        if (part) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) part[64 * half + i] = o[i];
+            part_ml[0] = m + kPackedP;               // (the products' sums are times 2^kPackedP)
+            part_ml[1] = l;
+        } else {
+            bf16* out = a.out + (size_t)tok * a.out_stride + (size_t)head * D + 64 * half;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) out[i] = __float2bfloat16_rn(o[i] / l);
+        }
+    }
+}
 
 template <int D, bool PACKED>
 __global__ void __launch_bounds__(threads<PACKED>(), 1)
@@ -276,6 +356,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     __shared__ volatile int tops_read[2 * kGroupThreads / 32];       // tiles whose words a softmax warp has taken
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int failed;
+    __shared__ volatile int far;                   // a tile's tokens are too far apart for float16
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // Blocks are handed out with x running fastest: the block's number in that order is cut so that all heads of
@@ -314,6 +395,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         for (int s = 0; PACKED && s < kTopRing; ++s) { tops[s] = 0u; tops_read[s] = 0; }
         for (int s = 0; s < kVStages; ++s) { mbar_init(&v_full[s], PACKED ? kUnpackWarps : 1); mbar_init(&v_empty[s], 1); }
         failed = 0;
+        far = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -366,19 +448,31 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                     }
                 }
             };
-            auto exponent = [&](const uint32_t (&u)[4][G], uint32_t least) {      // (a NaN, the sign of a token that was not finite, is passed over)
-                __nv_bfloat162 m = __float2bfloat162_rn(0.f);
+            auto exponent = [&](const uint32_t (&u)[4][G], uint32_t least, bool& apart) {      // (a NaN, the sign of a token that was not finite, is passed over)
+                uint32_t of[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i) {
+                    __nv_bfloat162 m = __float2bfloat162_rn(0.f);
 #pragma unroll
                     for (int g = 0; g < G; ++g) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u[i][g])));
-                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaf(15.f, __low2float(m), __high2float(m))));
-                return min(max(top >> 23, least), 254u);
+                    of[i] = __float_as_uint(fmaf(15.f, __low2float(m), __high2float(m)));
+                }
+                const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(of[0], of[1]), max(of[2], of[3])));
+                const uint32_t e8 = min(max(top >> 23, least), 254u);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) apart |= of[i] != 0u && (of[i] >> 23) + kReach < e8;
+                return e8;
             };
             fetch(0, table[quad_of(0) / ps]);
             if (n_tiles > 1) page = table[quad_of(1) / ps];
             for (int j = 0; j < n_tiles; ++j) {
-                const uint32_t word = exponent(par.k, kKeyLeast) | exponent(par.v, kValueLeast) << 8 | (uint32_t)(j + 1) << 16;
+                bool apart = false;
+                const uint32_t word = exponent(par.k, kKeyLeast, apart) | exponent(par.v, kValueLeast, apart) << 8 | (uint32_t)(j + 1) << 16;
+                if (apart) {                             // (known before the tile's word is)
+                    far = 1;
+                    __threadfence_block();
+                }
+                __syncwarp();
                 if (j + 1 < n_tiles) fetch(j + 1, page);
                 if (j + 2 < n_tiles) page = table[quad_of(j + 2) / ps];
                 bool read = false;                       // its slot's word has been taken by the softmax (the one behind it: by the unpacking too)
@@ -800,7 +894,13 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             if (lane == 0) mbar_arrive(&p_full[x]);              // one arrival per warp
         }
         if (ok && !mbar_wait(&o_done[x], 0)) { attn_give_up(8); failed = 1; ok = false; }
-        if (ok && !failed && eff_splits > 1) {
+        if (PACKED && ok && !failed && far) {
+            // (the products' result is dropped)
+            const size_t slot = (((size_t)tile_id * a.heads + head_a + x) * a.splits + split) * kRows + row;
+            if (row < rows)
+                attend_row<D>(a, tok0 + row, head_a + x, hk, req, max(k_begin, row_lo), min(k_begin + n_tiles * kKeys - 1, row_pos),
+                              eff_splits > 1 ? a.part_o + slot * kDim : nullptr, eff_splits > 1 ? a.part_ml + slot * 2 : nullptr);
+        } else if (ok && !failed && eff_splits > 1) {
             // partial result of this split: O as it stands (relative to m), and (m, l) of the row
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const size_t slot = ((size_t)tile_id * a.heads + head_a + x) * a.splits + split;
@@ -938,6 +1038,8 @@ int launch_prefill(const void* q, int q_stride, int tokens, const void* cache, l
     }
     AttnArgs a;
     a.packed = PACKED ? (const uint8_t*)cache : nullptr;
+    a.q = (const bf16*)q;
+    a.q_stride = q_stride;
     a.block_table = block_table;
     a.table_width = table_width;
     a.tiles = (const int4*)tiles;

@@ -15,10 +15,13 @@ a value v = z + s n, the mean square of an error of number c is then (U = 2^-8, 
   prompt portions  keys as float16                             sum_j p^2 H^2 / 3 scale^2 (sum_d q_d^2 k_d^2) (v - o)^2
                    p and values as float16                     2 sum_j p^2 H^2 / 3 v^2
                   and where float16 is not a matter of half steps relative to the number any more: keys and values lie in it over the
-                  power of two of the largest |z| + 15 s among a tile's 128 tokens (the largest becomes 2^14 to 2^15), so that s, z
-                  and z + s n are off by up to 2^-25 there, 17 2^-25 with fifteen steps; which is 17 2^-39 of the tile's largest:
-                  f = 17 2^-39 of the tile's largest key moves a score by up to f scale |q|_1, and the value's one adds up as it is.
-                  p times a tile's power is off by up to 2^-25 where the row's largest such product is 2^-1 at least: 2^-24 of that.
+                  power of two of the largest |z| + 15 s among a tile's 128 tokens (2^-67 and 2^-27 at least; the largest becomes
+                  2^14 to 2^15), so that s, z and z + s n are off by up to 2^-25 there, 17 2^-25 with fifteen steps, which is
+                  17 2^-39 of the tile's largest.  A tile with a token more than 2^22 below that is not worked on in float16 at all.
+                  For keys a score moves by up to 17 2^-39 scale |q|_1 of it, for values it adds up as it is.
+                  p times a tile's power, over the row's largest such product M, lies in float16 times 2^7: number v_j is off by up
+                  to 2^-25 2^-7 2 M |v_j| / (the tile's power).
+                  Results below 2^-126 are off by up to 2^-134.
 
 and the error of the row's head, as a vector, is allowed MARGIN times the root of the sum over its numbers.  The half step that a
 rounding takes is relative to the power of two below x, so (u x)^2 / 3 is twice the mean on average: three times the root are more than
@@ -39,15 +42,17 @@ def form_of(heads, kv, page, D, news):
     return "prompt", "single" if 32 % page == 0 or page % 32 == 0 else "general"
 
 
-def tiles_largest(z, s15, pos, first_query, window):
-    """[n] the largest |z| + 15 s among the 128 tokens of each token's tile that some query of the portion sees (z, 15 s: [n, D])."""
-    top = (z.abs() + s15).nan_to_num(nan=0.0).amax(-1)
-    if window:
-        top = torch.where(pos > first_query - window, top, 0.0)
-    out = torch.zeros_like(top)
-    for t in range(0, len(top), 128):
-        out[t:t + 128] = top[t:t + 128].max()
-    return out
+def tile_powers(z, s15, seen, least):
+    """([n] the largest |z| + 15 s among the tokens of each token's tile that the query tile sees, [n] whether the products work on that
+    tile in float16); z, 15 s: [n, D]."""
+    own = torch.where(seen, (z.abs() + s15).nan_to_num(nan=0.0).amax(-1), 0.0)
+    power, fine = torch.zeros_like(own), torch.ones_like(seen)
+    for t in range(0, len(own), 128):
+        tile = own[t:t + 128]
+        power[t:t + 128] = tile.max().clamp(min=least)
+        # (told apart by exponents: a token 2^22 to 2^23 below may count as either, and is off by as much as that)
+        fine[t:t + 128] = not bool(((tile > 0) & (tile * 2.0 ** 23 < power[t])).any())
+    return power, fine
 
 
 def attend(q, cache, table, lens, news, heads, kv, page, D, window=0, scale=0.0, wrong=None):
@@ -92,7 +97,7 @@ def attend(q, cache, table, lens, news, heads, kv, page, D, window=0, scale=0.0,
             def spread(w, x):                          # sum_c sum_j w_j (x_jc - r_c)^2
                 return w @ (x * x).sum(-1) - 2 * ((w @ x) * r).sum(-1) + w.sum(-1) * (r * r).sum(-1)
             p2 = p * p
-            var = U * U / 3 * (r * r).sum(-1)
+            var = U * U / 3 * (r * r).sum(-1) + D * 2.0 ** -268
             if form == "single":
                 var = var + H * H / 3 * spread(p2, v) + U * U / 3 * (p2 @ ((n_s - 8 * s) ** 2 + middle ** 2).sum(-1) + spread(p2, middle))
                 off = 2.0 ** -14 * scale * qh.abs().unflatten(-1, (-1, 32)).sum(-1) @ torch.where(unseen[:, None], 0.0, kstep[:, g]).T
@@ -100,16 +105,23 @@ def attend(q, cache, table, lens, news, heads, kv, page, D, window=0, scale=0.0,
             elif form == "prompt":
                 off = H * H / 3 * scale * scale * ((qh * qh) @ (k * k).T)
                 var = var + spread(p2 * off, v) + 2 * H * H / 3 * (p2 @ (v * v).sum(-1))
-                ktop, vtop = (tiles_largest(z[:, i, g], sn_max[:, i, g], pos, int(query[0]), window) for i in (0, 1))
-                moved = (17 * 2.0 ** -39 * scale) * qh.abs().sum(-1)[:, None] * ktop[None]
-                # weights that are off by a factor of up to e^moved; beyond that nothing is known but that they are weights
-                var = var + spread(p2 * torch.expm1(moved.clamp(max=1)) ** 2, v)
-                var = var + D * ((17 * 2.0 ** -39 * (p @ vtop)) ** 2 + total * (2.0 ** -24 * (p * vtop).amax(-1)) ** 2)
+                for r0 in range(0, new, 128):          # the kernel's query tiles
+                    at_rows = slice(r0, min(new, r0 + 128))
+                    lo, hi = int(query[r0]), int(query[at_rows][-1])
+                    seen = (pos <= hi) & (pos > lo - window if window else True)
+                    (kp, k_fine), (vp, v_fine) = (tile_powers(z[:, i, g], sn_max[:, i, g], seen, least) for i, least in ((0, 2.0 ** -67), (1, 2.0 ** -27)))
+                    fine = (k_fine & v_fine).double()
+                    pr = p[at_rows] * fine
+                    moved = (17 * 2.0 ** -39 * scale) * qh[at_rows].abs().sum(-1)[:, None] * kp[None]
+                    top = (pr * vp).amax(-1)
+                    var[at_rows] += (pr * pr * torch.expm1(moved.clamp(max=1)) ** 2) @ (v * v).sum(-1)
+                    var[at_rows] += D * (17 * 2.0 ** -39 * (pr @ vp)) ** 2
+                    var[at_rows] += (2.0 ** -31 * top) ** 2 * ((pr > 0).double() @ ((v * v).sum(-1) / vp ** 2))
             tol[:, h] = MARGIN * var.clamp(min=0).sqrt()
         rows.append(o)
         tols.append(tol)
         at += new
-    return torch.cat(rows), torch.cat(tols) + 1e-30
+    return torch.cat(rows), torch.cat(tols)
 
 
 def worst(got, want, tol):
