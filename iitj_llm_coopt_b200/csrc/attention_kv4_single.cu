@@ -10,9 +10,12 @@
 // another until the end.  A block takes one split of an item's tiles, dealt out in turn to its warps, and joins their sums; with more
 // than one split the blocks leave theirs in scratch memory, and a second kernel joins those.
 //
-// Measured, 32 heads over 8 of 128 numbers: 8 requests over 8192 tokens 30.8 us, 2.7 TB/s of codes (the reading alone would take 12.8);
-// 2 over 32768 tokens 31.8.  What bounds the loop now is the issue of instructions, about 720 a tile of 32 keys and 8 heads, half of
-// them integer ones, beside the matrix instructions' own time.
+// Measured, 32 heads over 8 of 128 numbers, over six inputs in turn: 8 requests over 8192 tokens 32.4 us, 2.6 TB/s of codes (the reading
+// alone would take 12.8); 2 over 32000 tokens 32.9; one over 4096 tokens 12.6, over 32000 25.4.  8 over 8192 of 64 numbers a head: 22.1.
+// What bounds it is not one thing.  Of 8 x 8192 a capture says: 950 instructions a tile of 32 keys and 8 heads with all that is around the
+// loop, which fill 51% of the issue slots of an SM while it works (ALU pipe 43%, tensor pipe 16%); 2.6 warps a scheduler, which wait for
+// what they need next rather than for a slot (stalls an issue: fixed latencies 0.89, loads 0.81, the pipes 0.49, shared memory 0.32); and a
+// fifth of the time in which an SM has nothing to do (256 blocks on 296 places: 40 SMs have one where the others have two).
 //
 //   scores   mma m16n8k16, 16 keys x 8 query heads.  A code n becomes the float16 1024 + n or 64 + n by one AND-OR (its last mantissa
 //            bits count 1 or 1/16), an exact number; q is float16 too, exactly, behind a power of two.  Per group of 32 the products' sum S
@@ -25,7 +28,8 @@
 //            numbers) and the sum of p are one more product, of rows of middles and of ones, with p as bfloat16.
 //            (About the zero points, with n for n - 8, the two parts nearly cancel over a long context: at 32000 keys the result was 5.2e-3
 //            off the one in 64 bits; it is 2.3e-3, of which bfloat16's last rounding alone makes 1.7e-3.  p and p s each rounded to
-//            bfloat16: 2.7e-3, and 30.8 us instead of 31.8.)
+//            bfloat16: 2.7e-3, and 30.8 us instead of 31.8.  Over contexts of 500 to 32000 tokens the result is 2.1e-3 to 2.4e-3 off: p s and
+//            the middles' p are each rounded by themselves, and the sum is of the latter.)
 //   range    p is up to 2^15 here, so p s would leave float32 and bfloat16 from steps of 2^113 on, and so would the products' 2^17 times a
 //            key's step.  From the first tile with a value's step or zero point of 2^65 or more a warp's sums are taken times 2^-64
 //            (its reference counts that); a tile with such a key has its stored words multiplied by 2^-64 where they lie in shared memory
@@ -46,7 +50,7 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)_
 constexpr int kTile = 32;               // keys of a warp's step
 // Six warps a block and two blocks an SM leave a thread 168 registers, which the two chains of the loop need (eight warps with 128:
 // 8 x 8192 keys at 32 / 8 heads of 128 in 33.5 us instead of 29.8; blocks of four, three an SM: 30.2 us, and 37 uneven contexts of 600
-// keys 17.4 us instead of 13.7; all before p s was rounded only once).
+// keys 17.4 us instead of 13.7; all before p s was rounded only once and before the words were looked at).
 constexpr int kWarps = 6, kResident = 2;
 constexpr float kStep = 8.f, kLift = 7.f;       // (log2 units) a reference's lag at most; p's factor
 constexpr int kHeads = 8;               // query heads of a block (columns of the products)

@@ -37,9 +37,12 @@
 //            largest product
 // A power holds the tokens of a tile down to 2^-22 of the largest.  Where one lies below that (or keys below 2^-89, values below 2^-49), a
 // query that sees it and not the loud one would lose it; the CTA then works its rows out one by one in float32 (attend_row).
-// Measured, 32 heads over 8 of 128 numbers: a prompt of 2048 tokens 62.7 us (over a bfloat16 cache 47), of 8192 tokens 651 us, 845
-// TFLOP/s (492 to 530).  Unpacking does not bound it: with the codes left as they are it took as long.  What it has more than the other form
-// is the maximum before the probabilities, the exponents, and registers: 14 warps leave a thread 128.
+// Measured, 32 heads over 8 of 128 numbers: a prompt of 2048 tokens 62.2 us (over a bfloat16 cache 47 to 50), of 8192 tokens 651 to 660
+// us, 835 TFLOP/s (492 to 545).  Unpacking does not bound it: with the codes left as they are it took as long.  What it has more than the
+// other form is the maximum before the probabilities, the exponents, and registers: 14 warps leave a thread 128.  At 2048 tokens a capture
+// says that 39% of the issue slots are filled and that the tensor pipe is at work a quarter of the time: the chain scores, maximum,
+// probabilities, product of two heads a tile is waited for (stalls an issue: loads, tensor memory's among them, 2.6, fixed latencies 1.5,
+// instruction fetch 1.3), and a sixth of the time an SM has no CTA any more.
 //
 // Every mbarrier wait is bounded; a wait that runs out records a code (llm_attention_tcgen05_status)
 // and the CTA falls through to its teardown, where the tensor memory is freed.

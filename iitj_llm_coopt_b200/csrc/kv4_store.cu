@@ -117,7 +117,8 @@ __device__ __forceinline__ void pack_group(const Eight& v, uint32_t& word, uint3
 }
 
 // grid (tokens, blocks of a token's warps).  A thread works on eight neighbouring numbers with 16-byte loads and stores.  Bound by
-// latency for a few rows (8 rows of 48 heads of 128: 2.5 us back to back); for many by the latency of a row's loads over the rows that
+// latency for a few rows (8 rows of 48 heads of 128: 2.5 us back to back; in place from 2, 4 or 8 partial sums, as a decode step stores
+// them, 3.5, 3.8 and 4.8); for many by the latency of a row's loads over the rows that
 // run at a time, half of memory's rate: 2048 rows (45 MB) 14.0 us, 8192 rows 46.8 us.  Five blocks an SM rather than four: 46.8 instead of
 // 51.2 us.  Four numbers a thread took 59.7 us, a loop over rows with the next row's numbers held in registers 106 us.
 template <typename T, bool PARTS>
@@ -203,8 +204,8 @@ rope_store_kv4_kernel(const Kv4StoreArgs a) {
 }
 
 // out[n][2][kv_heads][D] of the slots' keys and values: a thread per word of eight numbers.  A slot below 0 reads as zeros.  Bound by
-// the latency of slot -> word for a few slots, by memory for many (2048 slots of 8 heads of 128 to float32, 19 MB,
-// 5.5 us; 8192 slots 19.1 us); a block a slot took 30.6 us there.
+// the latency of slot -> word -> store, for many slots too (2048 slots of 8 heads of 128 to float32, 19 MB, 5.6 us, 3.0 at the rate of a
+// copy; 8192 slots 19.1 us, 62% of that rate); a block a slot took 30.6 us there.
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ slots, T* __restrict__ out, unsigned total, int kv_heads, int head_dim,
