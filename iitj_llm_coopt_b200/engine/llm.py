@@ -137,7 +137,7 @@ class LLM:
         one SamplingParams for all, or one per prompt.  `on_output(sequence, new_token_ids, finished)` is
         called as tokens arrive, as the reference's Sequence.on_output (engine/engine.py:40, 483-484).
         Returns RequestOutputs in order; a prompt whose SamplingParams ask for n completions has n of them, one after
-        the other, which share the prompt's cache pages."""
+        the other, which share the prompt's cache pages where they can (Engine.new_sequences)."""
         if prompt_token_ids and isinstance(prompt_token_ids[0], int):
             prompt_token_ids = [prompt_token_ids]
         n = len(prompt_token_ids)
